@@ -5,11 +5,16 @@ norms before and after a block with its gate and residual scale (ictc_o3.ops.blo
 operations.
 """
 import math
+import os
 import random
+import sys
 
 import torch
 
 own = False
+
+# The package root is a folder whose name is no module name: as the README says, on the path.
+sys.path.append(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "ictc-o3-hp-ascend_b200"))
 
 DEVICE = "cuda"
 BLOCK = 256                       # values that share one scale of an 8-bit state
