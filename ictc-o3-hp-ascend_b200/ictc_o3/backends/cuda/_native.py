@@ -12,11 +12,14 @@ import threading
 import torch
 
 LIBRARY_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libictc_cuda.so")
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
+_u64 = ctypes.c_uint64
+_f = ctypes.c_float
+_d = ctypes.c_double
 
 # name -> argtypes (all return int status unless listed in _RESTYPES)
 _SIGNATURES = {
@@ -57,10 +60,16 @@ _SIGNATURES = {
     "ictc_radial_pack": [_p, _p, _p, _p, _i, _i, _i, _p, _i64],
     "ictc_radial_forward": [_p, _p, _p, _i64, _i, _i, _i, _p, _p],
     "ictc_radial_backward": [_p, _p, _p, _p, _p, _i64, _i, _i, _i, _p, _p],
+    "ictc_adamw_chunk_values": [],
+    "ictc_adamw_workspace_bytes": [],
+    "ictc_adamw_grad_norm": [_p, _i, _p, _p, _f, _i, _i, _p, _p],
+    "ictc_adamw_step": [_p, _p, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _d, _u64, _i, _p,
+                        _p],
+    "ictc_adamw_decode": [_p, _p, _p, _p, _i64, _p, _p, _p],
 }
 _RESTYPES = {"ictc_last_error": ctypes.c_char_p, "ictc_sc_table_rows": _i64,
              "ictc_neighbor_workspace_bytes": _i64, "ictc_neighbor_noalloc_scratch_bytes": _i64,
-             "ictc_radial_image_bytes": _i64}
+             "ictc_radial_image_bytes": _i64, "ictc_adamw_workspace_bytes": _i64}
 
 _lock = threading.Lock()
 _lib = None

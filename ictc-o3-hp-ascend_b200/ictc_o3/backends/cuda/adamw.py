@@ -1,0 +1,74 @@
+"""AdamW kernels on the CUDA backend: static tables and launches of one optimizer.
+
+``TensorTable`` is what does not change while an optimizer lives: how its tensors are
+cut into chunks, and where each one's state lies (starts are multiples of
+``BLOCK`` values).  The addresses of weights and gradients are gathered for every step.
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from . import _native
+from ._native import ptr, stream_of
+
+BLOCK = 256   # values that share a scale of the 8-bit moments (csrc/adamw.cu)
+
+
+def blocks_of(numel: int) -> int:
+    return -(-numel // BLOCK)
+
+
+class TensorTable:
+    """Chunks and state places of tensors of the given sizes."""
+
+    def __init__(self, sizes, device):
+        chunk = int(_native.library().ictc_adamw_chunk_values())
+        sizes = torch.tensor(list(sizes), dtype=torch.int64)
+        blocks = (sizes + BLOCK - 1) // BLOCK
+        counts = (sizes + chunk - 1) // chunk
+        first = torch.zeros(sizes.numel() + 1, dtype=torch.int64)
+        torch.cumsum(counts, 0, out=first[1:])
+        starts = torch.cumsum(blocks, 0) - blocks
+        tensor = torch.repeat_interleave(torch.arange(sizes.numel()), counts)
+        number = torch.arange(int(first[-1])) - first[tensor]
+        if int(blocks.sum()) > 0x7fffffff:
+            raise ValueError("the optimizer holds too many values")
+        values = torch.clamp(sizes[tensor] - number * chunk, max=chunk)
+        block = starts[tensor] + number * (chunk // BLOCK)
+        table = torch.stack((tensor, values, block, number), 1).to(torch.int32)
+        self.count = sizes.numel()
+        self.starts = (starts * BLOCK).tolist()
+        self.blocks = int(blocks.sum())
+        self.values = self.blocks * BLOCK
+        self.chunks = table.contiguous().to(device)
+        self.first_chunk = (ctypes.c_int64 * (self.count + 1))(*first.tolist())
+        self.workspace = torch.zeros(int(_native.library().ictc_adamw_workspace_bytes()), dtype=torch.uint8,
+                                     device=device)
+        # word 2 of the workspace: gradient norm of the last step that computed one
+        self.norm = self.workspace[8:12].view(torch.float32)[0]
+
+    def grad_norm(self, grads, max_norm, skip_nonfinite):
+        """``grads``: address of a host array of ``count`` device pointers (0: no gradient)."""
+        _native.call("ictc_adamw_grad_norm", grads, self.count, ptr(self.chunks), self.first_chunk,
+                     1.0 if max_norm is None else max_norm, int(max_norm is not None), int(skip_nonfinite),
+                     ptr(self.workspace), stream_of(self.workspace))
+
+    def step(self, weights, grads, first, count, bits, state, *, lr, betas, eps, weight_decay, ema_decay, seed,
+             use_norm):
+        _native.call("ictc_adamw_step", weights, grads, first, count, ptr(self.chunks), self.first_chunk, bits,
+                     ptr(state["m"]), ptr(state["v"]), ptr(state["m_scale"]), ptr(state["v_scale"]),
+                     ptr(state["average"]), ptr(state["steps"]), lr, betas[0], betas[1], eps, weight_decay, ema_decay,
+                     seed, int(use_norm), ptr(self.workspace), stream_of(self.workspace))
+
+    def decode(self, state):
+        """BF16 values of the 8-bit moments."""
+        device = self.workspace.device
+        m = torch.empty(self.values, dtype=torch.bfloat16, device=device)
+        v = torch.empty(self.values, dtype=torch.bfloat16, device=device)
+        if self.values:
+            with torch.cuda.device(device):
+                _native.call("ictc_adamw_decode", ptr(state["m"]), ptr(state["v"]), ptr(state["m_scale"]),
+                             ptr(state["v_scale"]), self.values, ptr(m), ptr(v), stream_of(m))
+        return m, v

@@ -31,7 +31,7 @@
 extern "C" {
 #endif
 
-#define ICTC_ABI_VERSION 2
+#define ICTC_ABI_VERSION 3
 
 #define ICTC_OK 0
 #define ICTC_ERR_INVALID (-1)     /* bad pointer, size or shape            */
@@ -349,6 +349,47 @@ int ictc_wait_selftest(int* status, int64_t limit_ns, int arrive, void* stream);
 int64_t ictc_neighbor_noalloc_scratch_bytes(void);
 int ictc_neighbor_list_noalloc(const float* pos, int64_t atoms, const float* box, float cutoff, int64_t* offsets,
                                int64_t* src, int64_t* dst, float* shift, int64_t max_edges, void* stream);
+
+/*
+ * AdamW over a list of tensors (the optimizer of the reference's training step,
+ * mace_ictc/training/train_loop.py; its arithmetic is written out in csrc/adamw.cu).
+ *
+ * Static tables, built once by the caller:
+ *   chunks       device int32 [n][4]: every tensor is cut into chunks of
+ *                ictc_adamw_chunk_values() consecutive values (the last one shorter);
+ *                {tensor, values in the chunk, first 256-value block of the chunk in
+ *                the state arrays, number of the chunk inside its tensor}
+ *   first_chunk  host int64 [tensors + 1]: first chunk of every tensor
+ * State arrays hold the tensors one after another, each starting at a multiple of 256
+ * values and padded with zeros to one:
+ *   bits = 32  m, v FP32;  bits = 8  m, v one byte per value, m_scale, v_scale one
+ *   byte per 256 values;  average FP32 or NULL;  steps device int64 [tensors]
+ * `weights` and `grads` are host arrays of device pointers, read before the call
+ * returns; a NULL gradient leaves its tensor (and its step count) alone.
+ * `workspace`: ictc_adamw_workspace_bytes() device bytes, zeroed once, one per
+ * optimizer (two steps in flight must not share it).
+ *
+ * ictc_adamw_grad_norm puts |g| over all tensors, the clip factor
+ * min(1, max_norm / (|g| + 1e-6)) (1 unless clip) and, with skip_nonfinite, whether the
+ * step must be skipped into the workspace; word 2 of it is |g| (FP32).
+ * ictc_adamw_step updates tensors [first_tensor, first_tensor + tensors) of the same
+ * tables with one set of hyperparameters; use_norm != 0 applies what the last
+ * ictc_adamw_grad_norm found.  With bits = 8 a 256-value block whose new moments are
+ * not finite is left as it was.
+ */
+int ictc_adamw_chunk_values(void);
+int64_t ictc_adamw_workspace_bytes(void);
+int ictc_adamw_grad_norm(const void* const* grads, int tensors, const int32_t* chunks, const int64_t* first_chunk,
+                         float max_norm, int clip, int skip_nonfinite, void* workspace, void* stream);
+int ictc_adamw_step(void* const* weights, const void* const* grads, int first_tensor, int tensors,
+                    const int32_t* chunks, const int64_t* first_chunk, int bits, void* m, void* v, uint8_t* m_scale,
+                    uint8_t* v_scale, float* average, int64_t* steps, double lr, double beta1, double beta2,
+                    double eps, double weight_decay, double average_decay, uint64_t seed, int use_norm,
+                    void* workspace, void* stream);
+
+/* Values (BF16, exact) that 8-bit moments stand for; values is a multiple of 256. */
+int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_scale, const uint8_t* v_scale, int64_t values,
+                      void* m_out, void* v_out, void* stream);
 
 #ifdef __cplusplus
 }
