@@ -65,11 +65,17 @@ _SIGNATURES = {
     "ictc_adamw_grad_norm": [_p, _i, _p, _p, _f, _i, _i, _p, _p],
     "ictc_adamw_step": [_p, _p, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _d, _u64, _i, _p,
                         _p],
+    "ictc_block_partial_floats": [_i, _i],
+    "ictc_block_supported": [_i, _i],
+    "ictc_block_forward": [_p] * 6 + [_i, _i64, _i, _i, _i, _f] + [_p] * 5,
+    "ictc_block_backward": [_p] * 10 + [_i64, _i, _i, _i] + [_p] * 8,
+    "ictc_block_second": [_p] * 13 + [_i64, _i, _i, _i] + [_p] * 10,
     "ictc_adamw_decode": [_p, _p, _p, _p, _i64, _p, _p, _p],
 }
 _RESTYPES = {"ictc_last_error": ctypes.c_char_p, "ictc_sc_table_rows": _i64,
              "ictc_neighbor_workspace_bytes": _i64, "ictc_neighbor_noalloc_scratch_bytes": _i64,
-             "ictc_radial_image_bytes": _i64, "ictc_adamw_workspace_bytes": _i64}
+             "ictc_radial_image_bytes": _i64, "ictc_adamw_workspace_bytes": _i64,
+             "ictc_block_partial_floats": _i64}
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,113 @@
+"""Norms before and after a block, fused with the block's gate and residual scale.
+
+A stack of interaction and product blocks keeps a stream of node rows
+``[N, C (L+1)^2]`` (degrees 0..L, inside a degree ``mul_ir`` = [C][2l+1] or
+``ir_mul`` = [2l+1][C]).  With r(x) = (mean over a degree of x^2 + eps)^(-1/2), the end of one block and the
+start of the next are
+
+    stream' = stream + scale * sigmoid(gate) * post_weight * r(branch) * branch
+    normed  = pre_weight * r(stream') * stream'
+
+with weights and gates per degree and channel.  r depends on a degree's length only, so the
+operator commutes with rotations.  For lmax = 0 a row is a plain vector of C channels.
+Forward, first and second derivatives are one kernel each (forces and force-loss training
+need both); higher ones go through torch operations.
+"""
+from __future__ import annotations
+
+import torch
+
+from ictc_o3.backends.cuda.runtime import require_cuda_fp32
+
+__all__ = ["degree_norm", "residual_block_norm", "DegreeNorm", "ResidualBlockNorm"]
+
+
+def _form(channels, lmax, layout, eps, norm):
+    from ictc_o3.backends.cuda import _native
+    from ictc_o3.backends.cuda.block_norm import LAYOUTS, Form
+    if not isinstance(channels, int) or isinstance(channels, bool) or channels < 1:
+        raise ValueError("channels must be a positive integer")
+    if not isinstance(lmax, int) or isinstance(lmax, bool) or not 0 <= lmax <= 3:
+        raise ValueError("lmax must be 0, 1, 2 or 3")
+    if layout not in LAYOUTS:
+        raise ValueError("layout must be ir_mul or mul_ir")
+    if isinstance(eps, bool) or not isinstance(eps, (int, float)) or not 1.2e-38 <= eps < float("inf"):
+        raise ValueError("eps must be a positive FP32 number")
+    if not _native.library().ictc_block_supported(channels, lmax):
+        raise ValueError("rows of this width do not fit the kernels' shared memory")
+    return Form(channels, lmax, layout, float(eps), norm)
+
+
+def _check(form, rows, weights, gate=None):
+    n, c, width = rows[0].shape[0], form.channels, form.channels * (form.lmax + 1) ** 2
+    given = [w for w in weights if w is not None]
+    require_cuda_fp32(*rows, *given, *([] if gate is None else [gate]))
+    if any(x.ndim != 2 or x.shape != (n, width) for x in rows):
+        raise ValueError("Rows must have shape [N,C*(L+1)^2]")
+    if any(w.shape != (form.lmax + 1, c) for w in given):
+        raise ValueError("Weights must have shape [L+1,C]")
+    if gate is not None and gate.shape not in ((n, (form.lmax + 1) * c), (n, form.lmax + 1, c)):
+        raise ValueError("Gates must have shape [N,(L+1)*C] or [N,L+1,C]")
+
+
+def _contiguous(x):
+    return None if x is None else x.contiguous()
+
+
+def degree_norm(features, weight=None, *, channels, lmax, layout="mul_ir", eps=1e-6):
+    """weight * r(features) * features: the norm before the first block."""
+    from ictc_o3.backends.cuda.block_norm import _Block
+    form = _form(channels, lmax, layout, eps, True)
+    _check(form, [features], [weight])
+    return _Block.apply(form, features.contiguous(), None, None, None, None, _contiguous(weight))[0]
+
+
+def residual_block_norm(stream, branch, *, channels, lmax, post_weight=None, scale=None, gate=None, pre_weight=None,
+                        norm=None, layout="mul_ir", eps=1e-6):
+    """(stream', normed): the block's branch normed, gated, scaled and added, and the next block's norm.
+
+    Weights [L+1, C] (None: ones), gate [N, (L+1) C] before its sigmoid (None: no gate).  ``norm``:
+    whether the normed rows are wanted (default: when ``pre_weight`` is given); normed is None without."""
+    from ictc_o3.backends.cuda.block_norm import _Block
+    if norm is None:
+        norm = pre_weight is not None
+    if not isinstance(norm, bool) or (pre_weight is not None and not norm):
+        raise ValueError("norm must be a boolean, and true where pre_weight is given")
+    form = _form(channels, lmax, layout, eps, norm)
+    _check(form, [stream, branch], [post_weight, scale, pre_weight], gate)
+    if gate is not None:
+        gate = gate.reshape(gate.shape[0], (lmax + 1) * channels).contiguous()
+    out = _Block.apply(form, stream.contiguous(), branch.contiguous(), gate, _contiguous(post_weight),
+                       _contiguous(scale), _contiguous(pre_weight))
+    return out if norm else (out[0], None)
+
+
+class DegreeNorm(torch.nn.Module):
+    """``degree_norm`` with a weight per degree and channel."""
+
+    def __init__(self, channels, lmax, *, layout="mul_ir", eps=1e-6):
+        super().__init__()
+        self.channels, self.lmax, self.layout, self.eps = channels, lmax, layout, eps
+        self.weight = torch.nn.Parameter(torch.ones(lmax + 1, channels))
+
+    def forward(self, features):
+        return degree_norm(features, self.weight, channels=self.channels, lmax=self.lmax, layout=self.layout,
+                           eps=self.eps)
+
+
+class ResidualBlockNorm(torch.nn.Module):
+    """``residual_block_norm`` with its weights; ``next_norm`` False at the end of a stack.
+
+    ``scale_init`` is the branch's share at the start of training."""
+
+    def __init__(self, channels, lmax, *, next_norm=True, scale_init=1.0, layout="mul_ir", eps=1e-6):
+        super().__init__()
+        self.channels, self.lmax, self.layout, self.eps = channels, lmax, layout, eps
+        self.post_weight = torch.nn.Parameter(torch.ones(lmax + 1, channels))
+        self.scale = torch.nn.Parameter(torch.full((lmax + 1, channels), float(scale_init)))
+        self.pre_weight = torch.nn.Parameter(torch.ones(lmax + 1, channels)) if next_norm else None
+
+    def forward(self, stream, branch, gate=None):
+        return residual_block_norm(stream, branch, post_weight=self.post_weight, scale=self.scale, gate=gate,
+                                   pre_weight=self.pre_weight, channels=self.channels, lmax=self.lmax,
+                                   layout=self.layout, eps=self.eps)

@@ -391,6 +391,45 @@ int ictc_adamw_step(void* const* weights, const void* const* grads, int first_te
 int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_scale, const uint8_t* v_scale, int64_t values,
                       void* m_out, void* v_out, void* stream);
 
+/*
+ * Norms before and after a block with its gate and residual scale (no counterpart in
+ * the reference, whose stacks have two layers).  Rows [rows, C*(L+1)^2] of degrees
+ * 0..lmax (lmax <= 3) in layout 0 (ir_mul) or 1 (mul_ir); weights post, scale, pre
+ * [L+1, C] or NULL (= 1); gate [rows, (L+1)*C] or NULL.  Per row and degree
+ *   r(x) = (mean x^2 + eps)^(-1/2)
+ *   stream_out = stream + post * scale * sigmoid(gate) * r(branch) * branch
+ *   normed     = pre * r(stream_out) * stream_out                 (norm != 0)
+ * and with branch = NULL: normed = pre * r(stream) * stream.  r1, r2 [rows, L+1] receive
+ * r(branch) and r of the normed rows (NULL: not kept); the derivatives read them.
+ *
+ * ictc_block_backward: gradients for the cotangents p of stream_out and q of normed
+ * (either may be NULL: zero; q = NULL means no norm took part, the gradient of stream
+ * is then p itself and grad_stream must be NULL).  stream_out stands for stream
+ * where branch = NULL.  ictc_block_second: gradients of
+ * <dot_stream, grad_stream> + <dot_branch, grad_branch> + <dot_gate, grad_gate> with
+ * respect to (stream_out, branch, gate, post, scale, pre, p, q); a NULL dot is zero.
+ * Outputs that are NULL are not computed.  `partial`: ictc_block_partial_floats() device
+ * floats of scratch wherever a weight gradient is asked for.  Rows whose arrays are 16-byte
+ * aligned move as vectors; others give the same results.  ictc_block_supported tells
+ * whether rows of this width fit shared memory (up to 7,200 values do at any lmax).
+ */
+int64_t ictc_block_partial_floats(int channels, int lmax);
+int ictc_block_supported(int channels, int lmax);
+int ictc_block_forward(const float* stream_in, const float* branch, const float* gate, const float* post,
+                       const float* scale, const float* pre, int norm, int64_t rows, int channels, int lmax,
+                       int layout, float eps, float* stream_out, float* normed, float* r1, float* r2, void* stream);
+int ictc_block_backward(const float* stream_out, const float* branch, const float* gate, const float* post,
+                        const float* scale, const float* pre, const float* r1, const float* r2, const float* p,
+                        const float* q, int64_t rows, int channels, int lmax, int layout, float* grad_stream,
+                        float* grad_branch, float* grad_gate, float* grad_post, float* grad_scale, float* grad_pre,
+                        float* partial, void* stream);
+int ictc_block_second(const float* stream_out, const float* branch, const float* gate, const float* post,
+                      const float* scale, const float* pre, const float* r1, const float* r2, const float* p,
+                      const float* q, const float* dot_stream, const float* dot_branch, const float* dot_gate,
+                      int64_t rows, int channels, int lmax, int layout, float* grad_stream, float* grad_branch,
+                      float* grad_gate, float* grad_post, float* grad_scale, float* grad_pre, float* grad_p,
+                      float* grad_q, float* partial, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
