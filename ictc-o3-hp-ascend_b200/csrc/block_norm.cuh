@@ -1,0 +1,660 @@
+// Norms before and after a block, its gate and its residual scale, in one pass over the rows.
+//
+// A row holds degrees l = 0..L with C channels of 2l+1 components (C (L+1)^2 values; a degree
+// is [C][2l+1] or [2l+1][C]).  With D = C (2l+1) and <.,.> a degree's scalar product,
+//   r(x) = (<x,x> / D + eps)^(-1/2)
+//   h' = h + a r(y) y,  a = post scale sigma(gate)        per (degree, channel); gate optional
+//   u  = b r(h') h',    b = pre                           optional; without y: u of h itself
+// First gradients for cotangents p of h' and q of u, with n = r1 y, k = r2 h', D inside <.,.>
+// from here on (means):
+//   T  = p + r2 (b q - k <k, b q>)                        gradient of h
+//   dy = r1 (a T - n <n, a T>)
+//   S  = sum_m n T                                        per channel
+//   dgate = post scale sigma' S,  d(post scale) = sum_n sigma S,  db = sum_n sum_m k q
+// and <n, a T> = sum_c a S / D.  Second: cotangents al, be, ga of T, dy, dgate; with
+// inner = r1 (be - n <n,be>) and z = ga post scale sigma':
+//   tau = al + a inner + z n                              gradient of p
+//   gy  = r1^2 (3 n <n,aT> <n,be> - n <aT,be> - aT <n,be> - be <n,aT>) + r1 (z T - n <n,zT>)
+//   ga' = r1 (sum_m T be - <n,be> S)                      gradient of a, per channel
+//   g(post scale) = sum_n (sigma ga' + ga sigma' S),  ggate = post scale (sigma' ga' + ga sigma'' S)
+//   down = r2 (tau - k <k,tau>),  gq = b down,  gb = sum_n sum_m q down
+//   gh' = r2^2 (3 k <k,bq> <k,tau> - k <bq,tau> - bq <k,tau> - tau <k,bq>)
+// (written with n and k, not with powers of r: r^3 leaves FP32's range for rows of 1e13).
+//
+// All three are bound by the rows they read and write.  A lane owns one channel with all its
+// components, C lanes (one warp for several rows, or several warps for one) a row: sums over components
+// and per-channel values stay in a lane, weights and their gradients' sums in its registers, and
+// only the degrees' scalar products cross lanes.  A tile of rows is brought into shared memory by
+// asynchronous copies, one or more tiles ahead, read once, written back in place and leaves as contiguous
+// rows: a lane's channel lies 2l+1 values from its neighbour's, an odd stride, which shared
+// memory serves without conflicts and device memory would not.  Low degrees take several rows
+// per tile, so that a lane holds about 16 values of each tensor.  Rows wider than a
+// block's lanes (HOLD false) go over their channels in turns and read shared memory again
+// in every phase.  Weight gradients are summed per block and then over blocks by a second kernel, in
+// a fixed order: no atomics, the same bits every time.
+#pragma once
+
+#include "ictc_common.cuh"
+#include "ictc_cuda.h"
+
+#include <atomic>
+#include <cstdio>
+
+void ictc_set_error(const char* fmt, const char* detail);
+
+namespace ictc {
+namespace block_norm {
+
+constexpr int kMaxL = 3;
+constexpr int kMaxDevices = 64;
+constexpr int kSharedLimit = 227 * 1024;
+constexpr int kSharedBudget = 220 * 1024;
+
+enum Mode : int { kForward = 0, kBackward = 1, kSecond = 2 };
+
+// Staged tensors: 0..5 rows, then per-channel and per-degree ones.
+//   forward  y h . . . .      backward  y h' p q . .      second  y h' p q al be
+// (without a branch, the norm alone: . h, . h' . q, . h' . q al .)
+enum Slot : int { kY, kH, kP, kQ, kAl, kBe, kGate, kGateDot, kR1, kR2, kSlots };
+
+// Warps per block: what their registers leave room for (85, 128 and 255 of them).
+__host__ __device__ constexpr int max_warps(int mode) { return mode == kForward ? 24 : mode == kBackward ? 16 : 8; }
+// Warps of one row at most (a power of two).
+__host__ __device__ constexpr int max_row_warps(int mode) { return mode == kSecond ? 8 : 16; }
+// Rows that a lane works on at once.
+__host__ __device__ constexpr int rows_per_lane(int mode, int L, bool hold) {
+  return !hold ? 1 : mode == kSecond ? (L == 0 ? 4 : L == 1 ? 2 : 1) : (L == 0 ? 8 : L == 1 ? 4 : L == 2 ? 2 : 1);
+}
+constexpr int kScratch = 16;   // sums of one warp
+
+struct BlockArgs {
+  const float* in[kSlots];  // null: zeros, or not there
+  float* out[6];            // where rows go afterwards, or null
+  int at[kSlots];           // floats from the start of a stage, -1: no place
+  unsigned wide;            // bit s: tensor s is copied 16 bytes at a time
+  float* gate_out;          // dgate / its adjoint, or null
+  const float* post;        // [L+1, C] or null (1)
+  const float* scale;
+  const float* pre;
+  float* r1_out;            // [N, L+1], or null (forward)
+  float* r2_out;
+  float* partial;           // [blocks][2][(L+1) C] weight-gradient sums, or null
+  int64_t rows;
+  int channels;
+  int lanes;                // lanes per row
+  int warps;                // warps per group
+  int per;                  // rows of a tile
+  int stages;
+  int stage_floats;
+  int group_floats;
+  int norm;                 // u (or its cotangent) takes part
+  float eps;
+};
+
+struct Shape {
+  int hold, lanes, warps, per, stages, groups;
+};
+
+__device__ __forceinline__ void copy_async16(float* dst, const float* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copy_async4(float* dst, const float* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void copies_wait(int pending) {
+  if (pending >= 2) asm volatile("cp.async.wait_group 2;" ::: "memory");
+  else if (pending == 1) asm volatile("cp.async.wait_group 1;" ::: "memory");
+  else asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+
+// One warp (holding 32 / lanes rows at a time) or several warps of one row.
+struct Group {
+  int id;        // in the block
+  int thread;    // in the group
+  int threads;
+  int lanes;
+  float* scratch;   // two buffers, used in turn: one barrier per sum
+  int turn;
+
+  __device__ __forceinline__ void sync() const {
+    if (threads == 32) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
+  }
+  // Sums of N values over a row's lanes, in a fixed order, in every lane.
+  template <int N>
+  __device__ __forceinline__ void sum(float (&x)[N]) {
+    static_assert(N <= kScratch, "scratch");
+    const int top = lanes < 32 ? lanes : 32;
+    for (int o = top >> 1; o; o >>= 1) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
+    }
+    if (threads > 32) {
+      const int warps = threads >> 5;
+      float* s = scratch + turn * warps * kScratch;
+      turn ^= 1;
+      if ((thread & 31) == 0) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) s[(thread >> 5) * kScratch + i] = x[i];
+      }
+      sync();
+#pragma unroll
+      for (int i = 0; i < N; ++i) x[i] = 0.f;
+      for (int w = 0; w < warps; ++w) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) x[i] += s[w * kScratch + i];
+      }
+    }
+  }
+};
+
+// Values of one channel in R rows.
+template <int R, int L>
+struct Vals {
+  float v[R][(L + 1) * (L + 1)];
+};
+
+template <int L, int LAYOUT, int R>
+__device__ __forceinline__ void load(Vals<R, L>& x, const float* rows, int step, int C, int c) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int l = 0; l <= L; ++l)
+#pragma unroll
+      for (int m = 0; m < 2 * l + 1; ++m)
+        x.v[r][l * l + m] = rows[r * step + C * l * l + (LAYOUT == kMulIr ? c * (2 * l + 1) + m : m * C + c)];
+}
+template <int L, int LAYOUT, int R>
+__device__ __forceinline__ void store(const Vals<R, L>& x, float* rows, int step, int C, int c) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int l = 0; l <= L; ++l)
+#pragma unroll
+      for (int m = 0; m < 2 * l + 1; ++m)
+        rows[r * step + C * l * l + (LAYOUT == kMulIr ? c * (2 * l + 1) + m : m * C + c)] = x.v[r][l * l + m];
+}
+template <int R, int L>
+__device__ __forceinline__ void zero(Vals<R, L>& x) {
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int e = 0; e < (L + 1) * (L + 1); ++e) x.v[r][e] = 0.f;
+}
+
+// Channel weights of a lane: w = post scale, b = pre.
+template <int N>
+struct Weights {
+  float w[N], b[N];
+  __device__ __forceinline__ void load(const BlockArgs& a, int c) {
+#pragma unroll
+    for (int l = 0; l < N; ++l) {
+      const int at = l * a.channels + c;
+      w[l] = (a.post ? __ldg(a.post + at) : 1.f) * (a.scale ? __ldg(a.scale + at) : 1.f);
+      b[l] = a.pre ? __ldg(a.pre + at) : 1.f;
+    }
+  }
+};
+
+#define ICTC_ROWS(r, R) _Pragma("unroll") for (int r = 0; r < R; ++r)
+#define ICTC_DEGREES(l, N) _Pragma("unroll") for (int l = 0; l < N; ++l)
+#define ICTC_PARTS(e, l) _Pragma("unroll") for (int e = l * l; e < (l + 1) * (l + 1); ++e)
+
+template <int L, int LAYOUT, int MODE, bool BRANCH, bool HOLD>
+__global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __grid_constant__ BlockArgs a) {
+  extern __shared__ __align__(16) float shared[];
+  constexpr int N = L + 1, R = rows_per_lane(MODE, L, HOLD);
+  using V = Vals<R, L>;
+  const int C = a.channels, W = C * N * N, width = N * C;
+  Group g;
+  g.threads = 32 * a.warps;
+  g.id = threadIdx.x / g.threads;
+  g.thread = threadIdx.x % g.threads;
+  g.lanes = a.lanes;
+  g.turn = 0;
+  const int groups = blockDim.x / g.threads;
+  float* ring = shared + g.id * a.group_floats;
+  g.scratch = ring + a.stages * a.stage_floats;
+  float* acc = g.scratch + 2 * a.warps * kScratch;      // weight-gradient sums (HOLD false)
+  const int sub = g.thread / a.lanes;                   // this lane's rows are sub + r * (rows / R) of the tile
+  const int c0 = g.thread - sub * a.lanes;
+  const int apart = a.per / R;
+  const int64_t tiles = (a.rows + a.per - 1) / a.per;
+  const int64_t first = (int64_t)blockIdx.x * groups + g.id, stride = (int64_t)gridDim.x * groups;
+  if (!HOLD && a.partial)
+    for (int i = g.thread; i < 2 * width; i += g.threads) acc[i] = 0.f;
+
+  auto fetch = [&](int64_t t, int stage) {
+    if (t < tiles) {
+      const int64_t row0 = t * a.per;
+      const int rows = (int)(a.rows - row0 < a.per ? a.rows - row0 : a.per);
+      float* base = ring + stage * a.stage_floats;
+#pragma unroll
+      for (int s = 0; s < kSlots; ++s) {
+        if (a.in[s] == nullptr || a.at[s] < 0) continue;
+        const int wd = s < kGate ? W : s < kR1 ? width : N;
+        float* dst = base + a.at[s];
+        const float* src = a.in[s] + row0 * wd;
+        const int count = rows * wd;
+        int i = 0;
+        if (a.wide >> s & 1u) {
+#pragma unroll 4
+          for (int j = 4 * g.thread; j + 3 < count; j += 4 * g.threads) copy_async16(dst + j, src + j);
+          i = count & ~3;
+        }
+        for (i += g.thread; i < count; i += g.threads) copy_async4(dst + i, src + i);
+      }
+    }
+    copies_commit();
+  };
+  // f(c) for the lane's channels: one, or (HOLD false) several in turn.
+  auto each = [&](auto&& f) {
+    if constexpr (HOLD) {
+      if (c0 < C) f(c0);
+    } else {
+      for (int c = c0; c < C; c += a.lanes) f(c);
+    }
+  };
+
+  Weights<N> own;
+  float sum_w[N], sum_b[N];
+  ICTC_DEGREES(l, N) sum_w[l] = sum_b[l] = own.w[l] = own.b[l] = 0.f;
+  if (HOLD && c0 < C) own.load(a, c0);
+
+  for (int s = 0; s + 1 < a.stages; ++s) fetch(first + s * stride, s);
+  int stage = 0;
+  for (int64_t t = first; t < tiles; t += stride) {
+    if (a.stages == 1) {
+      g.sync();
+      fetch(t, 0);
+      copies_wait(0);
+      g.sync();
+    } else {
+      copies_wait(a.stages - 2);
+      g.sync();       // the tile is there, and everyone has left the stage that is filled next
+      fetch(t + (a.stages - 1) * stride, stage == 0 ? a.stages - 1 : stage - 1);
+    }
+    float* tile = ring + stage * a.stage_floats;
+    const int64_t row0 = t * a.per;
+    const int rows = (int)(a.rows - row0 < a.per ? a.rows - row0 : a.per);
+    bool real[R];
+    ICTC_ROWS(r, R) real[r] = sub + r * apart < rows;
+    const int step = apart * W;
+    auto at = [&](int s) { return tile + a.at[s] + sub * W; };
+    auto get = [&](V& x, int s, int c) { load<L, LAYOUT, R>(x, at(s), step, C, c); };
+    auto put = [&](const V& x, int s, int c) { store<L, LAYOUT, R>(x, at(s), step, C, c); };
+    auto rate = [&](float sum, int l) { return 1.f / sqrtf(sum / (float)(C * (2 * l + 1)) + a.eps); };
+    // a value per row, degree and channel (the widest rows leave no room for these)
+    auto channel = [&](int s, int r, int l, int c) {
+      return HOLD ? tile[a.at[s] + (sub + r * apart) * width + l * C + c] : __ldg(a.in[s] + row0 * width + l * C + c);
+    };
+    // sigma(gate) of a channel, per row and degree
+    auto sigma = [&](float (&s)[R][N], int c) {
+      ICTC_ROWS(r, R) ICTC_DEGREES(l, N)
+        s[r][l] = a.in[kGate] ? 1.f / (1.f + expf(-channel(kGate, r, l, c))) : 1.f;
+    };
+    auto weights = [&](int c) {
+      if constexpr (!HOLD) own.load(a, c);
+    };
+    // HOLD false: a phase starts by reading again what an earlier one read or wrote
+    auto again = [&](V& x, int s, int c) {
+      if constexpr (!HOLD) get(x, s, c);
+    };
+
+    if constexpr (MODE == kForward) {
+      V y, h;
+      float r1[R][N], s[R * N];
+      if constexpr (BRANCH) {
+        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) s[r * N + l] = 0.f;
+        each([&](int c) {
+          get(y, kY, c);
+          ICTC_ROWS(r, R) ICTC_DEGREES(l, N) ICTC_PARTS(e, l) s[r * N + l] = fmaf(y.v[r][e], y.v[r][e], s[r * N + l]);
+        });
+        g.sum(s);
+        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) r1[r][l] = rate(s[r * N + l], l);
+        if (a.r1_out && c0 == 0)
+          ICTC_ROWS(r, R) if (real[r]) ICTC_DEGREES(l, N)
+            a.r1_out[(row0 + sub + r * apart) * N + l] = r1[r][l];
+      }
+      ICTC_ROWS(r, R) ICTC_DEGREES(l, N) s[r * N + l] = 0.f;
+      each([&](int c) {
+        get(h, kH, c);
+        if constexpr (BRANCH) {
+          again(y, kY, c);
+          weights(c);
+          float sg[R][N];
+          sigma(sg, c);
+          ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+            const float f = own.w[l] * sg[r][l] * r1[r][l];
+            ICTC_PARTS(e, l) h.v[r][e] = fmaf(f, y.v[r][e], h.v[r][e]);
+          }
+          put(h, kH, c);
+        }
+        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) ICTC_PARTS(e, l) s[r * N + l] = fmaf(h.v[r][e], h.v[r][e], s[r * N + l]);
+      });
+      if (a.norm) {
+        g.sum(s);
+        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) s[r * N + l] = rate(s[r * N + l], l);
+        if (a.r2_out && c0 == 0)
+          ICTC_ROWS(r, R) if (real[r]) ICTC_DEGREES(l, N)
+            a.r2_out[(row0 + sub + r * apart) * N + l] = s[r * N + l];
+        each([&](int c) {
+          again(h, kH, c);
+          weights(c);
+          ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+            const float f = own.b[l] * s[r * N + l];
+            ICTC_PARTS(e, l) h.v[r][e] *= f;
+          }
+          put(h, kY, c);
+        });
+      }
+    } else {
+      V h, q, T, y;
+      float r1[R][N], r2[R][N], kq[R * N];
+      ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+        const int from = (sub + r * apart) * N + l;
+        r1[r][l] = BRANCH ? tile[a.at[kR1] + from] : 0.f;
+        r2[r][l] = a.norm ? tile[a.at[kR2] + from] : 0.f;
+        kq[r * N + l] = 0.f;
+      }
+      if (a.norm) {
+        each([&](int c) {
+          get(h, kH, c);
+          get(q, kQ, c);
+          weights(c);
+          ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+            float s = 0.f;
+            ICTC_PARTS(e, l) s = fmaf(r2[r][l] * h.v[r][e], q.v[r][e], s);
+            kq[r * N + l] = fmaf(own.b[l], s, kq[r * N + l]);
+            if (MODE == kBackward && real[r]) {
+              if constexpr (HOLD) sum_b[l] += s;
+              else if (a.partial) acc[width + l * C + c] += s;
+            }
+          }
+        });
+        g.sum(kq);
+        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) kq[r * N + l] /= (float)(C * (2 * l + 1));      // <k, b q>
+      }
+      // T = p + r2 (b q - k <k, b q>)
+      auto total = [&](int c) {
+        if constexpr (BRANCH) {
+          if (a.in[kP]) get(T, kP, c);
+          else zero(T);
+        } else {
+          zero(T);
+        }
+        weights(c);
+        if (a.norm) {
+          again(h, kH, c);
+          again(q, kQ, c);
+          ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+            const float f = r2[r][l] * kq[r * N + l];
+            ICTC_PARTS(e, l) T.v[r][e] = fmaf(r2[r][l], own.b[l] * q.v[r][e] - f * h.v[r][e], T.v[r][e]);
+          }
+        }
+      };
+      if constexpr (MODE == kBackward) {
+        float nT[R * N];
+        float sg[R][N];
+        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) nT[r * N + l] = 0.f;
+        each([&](int c) {
+          total(c);
+          if (a.out[BRANCH ? kP : kQ] || !HOLD) put(T, BRANCH ? kP : kQ, c);
+          if constexpr (BRANCH) {
+            get(y, kY, c);
+            sigma(sg, c);
+            ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+              float S = 0.f;
+              ICTC_PARTS(e, l) S = fmaf(r1[r][l] * y.v[r][e], T.v[r][e], S);
+              nT[r * N + l] = fmaf(own.w[l] * sg[r][l], S, nT[r * N + l]);
+              if (real[r]) {
+                if (a.gate_out)
+                  a.gate_out[(row0 + sub + r * apart) * width + l * C + c] =
+                      own.w[l] * sg[r][l] * (1.f - sg[r][l]) * S;
+                if constexpr (HOLD) sum_w[l] = fmaf(sg[r][l], S, sum_w[l]);
+                else if (a.partial) acc[l * C + c] += sg[r][l] * S;
+              }
+            }
+          }
+        });
+        if constexpr (BRANCH) {
+          if (a.out[kY]) {
+            g.sum(nT);
+            each([&](int c) {
+              if constexpr (!HOLD) {
+                get(T, kP, c);
+                get(y, kY, c);
+                weights(c);
+                sigma(sg, c);
+              }
+              ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+                const float f = r1[r][l] * nT[r * N + l] / (float)(C * (2 * l + 1)), aw = own.w[l] * sg[r][l];
+                ICTC_PARTS(e, l) y.v[r][e] = r1[r][l] * (aw * T.v[r][e] - f * y.v[r][e]);
+              }
+              put(y, kY, c);
+            });
+          }
+        }
+      } else {
+        V be, tau;
+        float sg[R][N], dt[R][N], k[4 * R * N];      // <n,aT>, <n,be>, <aT,be>, <n,zT>
+        auto dots = [&](int c) {
+          ICTC_ROWS(r, R) ICTC_DEGREES(l, N)
+            dt[r][l] = a.in[kGateDot] ? channel(kGateDot, r, l, c) : 0.f;
+        };
+        if constexpr (BRANCH) {
+#pragma unroll
+          for (int i = 0; i < 4 * R * N; ++i) k[i] = 0.f;
+          each([&](int c) {
+            total(c);
+            if constexpr (!HOLD) put(T, kP, c);
+            get(y, kY, c);
+            if (a.in[kBe]) get(be, kBe, c);
+            else zero(be);
+            sigma(sg, c);
+            dots(c);
+            ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+              float S = 0.f, nb = 0.f, tb = 0.f;
+              ICTC_PARTS(e, l) {
+                const float n = r1[r][l] * y.v[r][e];
+                S = fmaf(n, T.v[r][e], S);
+                nb = fmaf(n, be.v[r][e], nb);
+                tb = fmaf(T.v[r][e], be.v[r][e], tb);
+              }
+              float* kk = k + 4 * (r * N + l);
+              const float aw = own.w[l] * sg[r][l];
+              kk[0] = fmaf(aw, S, kk[0]);
+              kk[1] += nb;
+              kk[2] = fmaf(aw, tb, kk[2]);
+              kk[3] = fmaf(dt[r][l] * aw * (1.f - sg[r][l]), S, kk[3]);
+            }
+          });
+          g.sum(k);
+          ICTC_ROWS(r, R) ICTC_DEGREES(l, N)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) k[4 * (r * N + l) + i] /= (float)(C * (2 * l + 1));
+        }
+        float kt[2 * R * N];                         // <k,tau>, <bq,tau>
+#pragma unroll
+        for (int i = 0; i < 2 * R * N; ++i) kt[i] = 0.f;
+        each([&](int c) {
+          if (a.in[kAl]) get(tau, kAl, c);
+          else zero(tau);
+          weights(c);
+          if constexpr (BRANCH) {
+            if constexpr (!HOLD) {
+              get(T, kP, c);
+              get(y, kY, c);
+              if (a.in[kBe]) get(be, kBe, c);
+              else zero(be);
+              sigma(sg, c);
+              dots(c);
+            }
+            ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+              const float* kk = k + 4 * (r * N + l);
+              const float r0 = r1[r][l], nT = kk[0], nb = kk[1], Tb = kk[2], nz = kk[3];
+              const float slope = sg[r][l] * (1.f - sg[r][l]), aw = own.w[l] * sg[r][l];
+              const float z = dt[r][l] * own.w[l] * slope;
+              // gy = cn n + ct T + cb be
+              const float cn = r0 * (r0 * (3.f * nT * nb - Tb) - nz), ct = r0 * (z - r0 * nb * aw), cb = -r0 * r0 * nT;
+              float S = 0.f, tb = 0.f;
+              ICTC_PARTS(e, l) {
+                const float n = r0 * y.v[r][e], tv = T.v[r][e], bv = be.v[r][e];
+                S = fmaf(n, tv, S);
+                tb = fmaf(tv, bv, tb);
+                tau.v[r][e] += aw * r0 * (bv - nb * n) + z * n;
+                y.v[r][e] = cn * n + ct * tv + cb * bv;
+              }
+              const float ga = r0 * (tb - nb * S);
+              if (real[r]) {
+                if (a.gate_out)
+                  a.gate_out[(row0 + sub + r * apart) * width + l * C + c] =
+                      own.w[l] * slope * (ga + dt[r][l] * (1.f - 2.f * sg[r][l]) * S);
+                const float gw = sg[r][l] * ga + dt[r][l] * slope * S;
+                if constexpr (HOLD) sum_w[l] += gw;
+                else if (a.partial) acc[l * C + c] += gw;
+              }
+            }
+            if (a.out[kY]) put(y, kY, c);
+          }
+          if (BRANCH || !HOLD) put(tau, kAl, c);
+          if (a.norm) {
+            again(h, kH, c);
+            again(q, kQ, c);
+            ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+              float* kk = kt + 2 * (r * N + l);
+              float qt = 0.f;
+              ICTC_PARTS(e, l) {
+                kk[0] = fmaf(r2[r][l] * h.v[r][e], tau.v[r][e], kk[0]);
+                qt = fmaf(q.v[r][e], tau.v[r][e], qt);
+              }
+              kk[1] = fmaf(own.b[l], qt, kk[1]);
+            }
+          }
+        });
+        if (a.norm) {
+          g.sum(kt);
+          each([&](int c) {
+            if constexpr (!HOLD) {
+              get(tau, kAl, c);
+              get(h, kH, c);
+              get(q, kQ, c);
+              weights(c);
+            }
+            ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
+              const float inv = 1.f / (float)(C * (2 * l + 1)), r0 = r2[r][l], b = own.b[l];
+              const float kt0 = kt[2 * (r * N + l)] * inv, qt = kt[2 * (r * N + l) + 1] * inv, kq0 = kq[r * N + l];
+              const float ck = r0 * r0 * (3.f * kq0 * kt0 - qt);
+              float gb = 0.f;
+              ICTC_PARTS(e, l) {
+                const float kv = r0 * h.v[r][e], qv = q.v[r][e], tv = tau.v[r][e];
+                const float down = r0 * (tv - kt0 * kv);
+                gb = fmaf(qv, down, gb);
+                q.v[r][e] = b * down;
+                h.v[r][e] = ck * kv - r0 * r0 * (kt0 * b * qv + kq0 * tv);
+              }
+              if (real[r]) {
+                if constexpr (HOLD) sum_b[l] += gb;
+                else if (a.partial) acc[width + l * C + c] += gb;
+              }
+            }
+            put(h, kH, c);
+            put(q, kQ, c);
+          });
+        }
+      }
+    }
+    g.sync();
+#pragma unroll
+    for (int s = 0; s < 6; ++s) {
+      // forward: u leaves from y's place
+      if (a.out[s] == nullptr) continue;
+      float* dst = a.out[s] + row0 * W;
+      const float* src = tile + a.at[s];
+      const int count = rows * W;
+      int i = 0;
+      if (a.wide >> (16 + s) & 1u) {
+#pragma unroll 4
+        for (int j = 4 * g.thread; j + 3 < count; j += 4 * g.threads)
+          *reinterpret_cast<float4*>(dst + j) = *reinterpret_cast<const float4*>(src + j);
+        i = count & ~3;
+      }
+      for (i += g.thread; i < count; i += g.threads) dst[i] = src[i];
+    }
+    stage = stage + 1 == a.stages ? 0 : stage + 1;
+  }
+  if (a.partial == nullptr) return;
+  // Sums of the block's groups (and of a warp's rows side by side), in order.
+  __syncthreads();
+  const int beside = 32 * a.warps / a.lanes;      // rows side by side in a group
+  if constexpr (HOLD) {
+    float* mine = shared + (int64_t)(g.id * beside + sub) * 2 * width;
+    if (c0 < C) ICTC_DEGREES(l, N) {
+      mine[l * C + c0] = sum_w[l];
+      mine[width + l * C + c0] = sum_b[l];
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 2 * width; i += blockDim.x) {
+    float s = 0.f;
+    if constexpr (HOLD) {
+      for (int k = 0; k < groups * beside; ++k) s += shared[(int64_t)k * 2 * width + i];
+    } else {
+      for (int k = 0; k < groups; ++k)
+        s += shared[k * a.group_floats + a.stages * a.stage_floats + 2 * a.warps * kScratch + i];
+    }
+    a.partial[(int64_t)blockIdx.x * 2 * width + i] = s;
+  }
+}
+
+template <int L, int LAYOUT, int MODE, bool BRANCH, bool HOLD>
+cudaError_t launch_one(const BlockArgs& a, const Shape& s, int grid, int shared_bytes, cudaStream_t stream) {
+  auto kernel = block_kernel<L, LAYOUT, MODE, BRANCH, HOLD>;
+  static std::atomic<bool> ready[kMaxDevices];   // shared-memory limit raised on this device
+  int device = 0;
+  cudaError_t err = cudaGetDevice(&device);
+  if (err != cudaSuccess) return err;
+  if (device >= kMaxDevices || !ready[device].load(std::memory_order_relaxed)) {
+    err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedLimit);
+    if (err != cudaSuccess) return err;
+    if (device < kMaxDevices) ready[device].store(true, std::memory_order_relaxed);
+  }
+  kernel<<<grid, s.groups * s.warps * 32, shared_bytes, stream>>>(a);
+  return cudaGetLastError();
+}
+
+template <int L, int MODE, bool BRANCH>
+cudaError_t launch_layout(const BlockArgs& a, const Shape& s, int grid, int bytes, int layout, cudaStream_t stream) {
+  if (layout == kMulIr)
+    return s.hold ? launch_one<L, kMulIr, MODE, BRANCH, true>(a, s, grid, bytes, stream)
+                  : launch_one<L, kMulIr, MODE, BRANCH, false>(a, s, grid, bytes, stream);
+  return s.hold ? launch_one<L, kIrMul, MODE, BRANCH, true>(a, s, grid, bytes, stream)
+                : launch_one<L, kIrMul, MODE, BRANCH, false>(a, s, grid, bytes, stream);
+}
+template <int MODE, bool BRANCH>
+cudaError_t launch_degree(const BlockArgs& a, const Shape& s, int grid, int bytes, int lmax, int layout,
+                          cudaStream_t stream) {
+  switch (lmax) {
+    case 0: return launch_layout<0, MODE, BRANCH>(a, s, grid, bytes, layout, stream);
+    case 1: return launch_layout<1, MODE, BRANCH>(a, s, grid, bytes, layout, stream);
+    case 2: return launch_layout<2, MODE, BRANCH>(a, s, grid, bytes, layout, stream);
+    default: return launch_layout<3, MODE, BRANCH>(a, s, grid, bytes, layout, stream);
+  }
+}
+template <int MODE>
+cudaError_t launch_mode(const BlockArgs& a, const Shape& s, int grid, int bytes, int lmax, int layout, bool branch,
+                        cudaStream_t stream) {
+  return branch ? launch_degree<MODE, true>(a, s, grid, bytes, lmax, layout, stream)
+                : launch_degree<MODE, false>(a, s, grid, bytes, lmax, layout, stream);
+}
+
+// One per mode, each in a file of its own (they compile side by side).
+cudaError_t launch_forward(const BlockArgs&, const Shape&, int, int, int, int, bool, cudaStream_t);
+cudaError_t launch_backward(const BlockArgs&, const Shape&, int, int, int, int, bool, cudaStream_t);
+cudaError_t launch_second(const BlockArgs&, const Shape&, int, int, int, int, bool, cudaStream_t);
+
+}  // namespace block_norm
+}  // namespace ictc
