@@ -120,6 +120,7 @@ int run(int mode, BlockArgs& a, int lmax, int layout, bool branch, int* blocks, 
     if (aligned(a.in[k])) a.wide |= 1u << k;
     if (k < 6 && aligned(a.out[k])) a.wide |= 1u << (16 + k);
   }
+  for (int l = 0; l < N; ++l) a.inv[l] = (float)(1.0 / ((double)C * (2 * l + 1)));
   a.lanes = s.lanes;
   a.warps = s.warps;
   a.per = s.per;

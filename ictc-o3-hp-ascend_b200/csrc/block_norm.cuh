@@ -89,6 +89,7 @@ struct BlockArgs {
   int group_floats;
   int norm;                 // u (or its cotangent) takes part
   float eps;
+  float inv[kMaxL + 1];     // 1 / D of every degree
 };
 
 struct Shape {
@@ -123,33 +124,71 @@ struct Group {
     if (threads == 32) __syncwarp();
     else asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
   }
-  // Sums of N values over a row's lanes, in a fixed order, in every lane.
+  // Sums of N values over a row's lanes, in a fixed order, in every lane.  Over whole warps
+  // each exchange halves the values that a lane carries on (N - 1 + 5 - log2 N exchanges
+  // instead of 5 N); the sums then go round through shared memory, as they must between warps.
   template <int N>
   __device__ __forceinline__ void sum(float (&x)[N]) {
     static_assert(N <= kScratch, "scratch");
-    const int top = lanes < 32 ? lanes : 32;
-    for (int o = top >> 1; o; o >>= 1) {
+    if (lanes < 32) {
+      for (int o = lanes >> 1; o; o >>= 1) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
-    }
-    if (threads > 32) {
-      const int warps = threads >> 5;
-      float* s = scratch + turn * warps * kScratch;
-      turn ^= 1;
-      if ((thread & 31) == 0) {
-#pragma unroll
-        for (int i = 0; i < N; ++i) s[(thread >> 5) * kScratch + i] = x[i];
+        for (int i = 0; i < N; ++i) x[i] += __shfl_xor_sync(0xffffffffu, x[i], o);
       }
-      sync();
+      return;
+    }
+    constexpr int P = N > 8 ? 16 : N > 4 ? 8 : N > 2 ? 4 : N;
+    float v[P];
 #pragma unroll
-      for (int i = 0; i < N; ++i) x[i] = 0.f;
-      for (int w = 0; w < warps; ++w) {
+    for (int i = 0; i < P; ++i) v[i] = i < N ? x[i] : 0.f;
+    const int lane = thread & 31;
+    int index = 0;
 #pragma unroll
-        for (int i = 0; i < N; ++i) x[i] += s[w * kScratch + i];
+    for (int step = 0; step < 5; ++step) {
+      const int o = 16 >> step, half = P >> (step + 1);
+      if (half > 0) {
+        const bool upper = lane & o;
+        index += upper ? half : 0;
+#pragma unroll
+        for (int i = 0; i < half; ++i) {
+          const float keep = upper ? v[i + half] : v[i], give = upper ? v[i] : v[i + half];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, give, o);
+        }
+      } else {
+        v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+      }
+    }
+    const int warps = threads >> 5;
+    float* s = scratch + turn * warps * kScratch;
+    turn ^= 1;
+    if ((lane & (32 / P - 1)) == 0) s[(thread >> 5) * kScratch + index] = v[0];
+    sync();
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = 0.f;
+    for (int w = 0; w < warps; ++w) {
+#pragma unroll
+      for (int i = 0; i < N; i += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(s + w * kScratch + i);
+        x[i] += t.x;
+        if (i + 1 < N) x[i + 1] += t.y;
+        if (i + 2 < N) x[i + 2] += t.z;
+        if (i + 3 < N) x[i + 3] += t.w;
       }
     }
   }
 };
+
+// 1 / (1 + exp(-g)) from the hardware's 2^x and quotient, with the rounding of g log2(e) put
+// back (2^x alone is off by |g| half steps).
+__device__ __forceinline__ float sigmoid(float g) {
+  constexpr float kLog2e = 1.4426950408889634f, kLog2eRest = 1.9259629911266175e-8f;
+  const float t = -g * kLog2e;
+  const float rest = (fmaf(-g, kLog2e, -t) - g * kLog2eRest) * 0.6931471805599453f;
+  float e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(t));
+  if (fabsf(t) < 126.f) e = fmaf(e, rest, e);     // beyond, 0 and infinity stay what they are
+  return __fdividef(1.f, 1.f + e);
+}
 
 // Values of one channel in R rows.
 template <int R, int L>
@@ -286,7 +325,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
     auto at = [&](int s) { return tile + a.at[s] + sub * W; };
     auto get = [&](V& x, int s, int c) { load<L, LAYOUT, R>(x, at(s), step, C, c); };
     auto put = [&](const V& x, int s, int c) { store<L, LAYOUT, R>(x, at(s), step, C, c); };
-    auto rate = [&](float sum, int l) { return 1.f / sqrtf(sum / (float)(C * (2 * l + 1)) + a.eps); };
+    auto rate = [&](float sum, int l) { return rsqrtf(fmaf(sum, a.inv[l], a.eps)); };
     // a value per row, degree and channel (the widest rows leave no room for these)
     auto channel = [&](int s, int r, int l, int c) {
       return HOLD ? tile[a.at[s] + (sub + r * apart) * width + l * C + c] : __ldg(a.in[s] + row0 * width + l * C + c);
@@ -294,7 +333,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
     // sigma(gate) of a channel, per row and degree
     auto sigma = [&](float (&s)[R][N], int c) {
       ICTC_ROWS(r, R) ICTC_DEGREES(l, N)
-        s[r][l] = a.in[kGate] ? 1.f / (1.f + expf(-channel(kGate, r, l, c))) : 1.f;
+        s[r][l] = a.in[kGate] ? sigmoid(channel(kGate, r, l, c)) : 1.f;
     };
     auto weights = [&](int c) {
       if constexpr (!HOLD) own.load(a, c);
@@ -376,7 +415,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
           }
         });
         g.sum(kq);
-        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) kq[r * N + l] /= (float)(C * (2 * l + 1));      // <k, b q>
+        ICTC_ROWS(r, R) ICTC_DEGREES(l, N) kq[r * N + l] *= a.inv[l];      // <k, b q>
       }
       // T = p + r2 (b q - k <k, b q>)
       auto total = [&](int c) {
@@ -431,7 +470,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
                 sigma(sg, c);
               }
               ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
-                const float f = r1[r][l] * nT[r * N + l] / (float)(C * (2 * l + 1)), aw = own.w[l] * sg[r][l];
+                const float f = r1[r][l] * nT[r * N + l] * a.inv[l], aw = own.w[l] * sg[r][l];
                 ICTC_PARTS(e, l) y.v[r][e] = r1[r][l] * (aw * T.v[r][e] - f * y.v[r][e]);
               }
               put(y, kY, c);
@@ -475,7 +514,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
           g.sum(k);
           ICTC_ROWS(r, R) ICTC_DEGREES(l, N)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) k[4 * (r * N + l) + i] /= (float)(C * (2 * l + 1));
+            for (int i = 0; i < 4; ++i) k[4 * (r * N + l) + i] *= a.inv[l];
         }
         float kt[2 * R * N];                         // <k,tau>, <bq,tau>
 #pragma unroll
@@ -545,7 +584,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
               weights(c);
             }
             ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
-              const float inv = 1.f / (float)(C * (2 * l + 1)), r0 = r2[r][l], b = own.b[l];
+              const float inv = a.inv[l], r0 = r2[r][l], b = own.b[l];
               const float kt0 = kt[2 * (r * N + l)] * inv, qt = kt[2 * (r * N + l) + 1] * inv, kq0 = kq[r * N + l];
               const float ck = r0 * r0 * (3.f * kq0 * kt0 - qt);
               float gb = 0.f;
