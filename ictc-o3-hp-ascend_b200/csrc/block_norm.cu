@@ -33,7 +33,7 @@ __global__ void __launch_bounds__(256) weight_sum_kernel(const float* __restrict
 // the places of the staged tensors (`there`: bit per slot).
 bool shape_of(int C, int L, int mode, unsigned there, bool sums, int64_t rows, int sms, Shape* s, BlockArgs* a,
               int* shared_bytes) {
-  const int N = L + 1, most_row = max_row_warps(mode);
+  const int N = L + 1, most_row = max_row_warps(mode, L);
   const int64_t W = (int64_t)C * N * N;
   if (W > (1 << 16)) return false;
   s->hold = C <= 32 * most_row;
@@ -42,7 +42,7 @@ bool shape_of(int C, int L, int mode, unsigned there, bool sums, int64_t rows, i
   if (C <= 32) {
     while (s->lanes < C) s->lanes *= 2;
   } else {
-    while (s->warps < most_row && 32 * s->warps < C) s->warps *= 2;
+    s->warps = (C + 31) / 32 < most_row ? (C + 31) / 32 : most_row;
     s->lanes = 32 * s->warps;
   }
   const int beside = 32 * s->warps / s->lanes;
@@ -52,11 +52,11 @@ bool shape_of(int C, int L, int mode, unsigned there, bool sums, int64_t rows, i
     a->at[k] = -1;
     if (!(there >> k & 1u) || (!s->hold && (k == kGate || k == kGateDot))) continue;
     a->at[k] = (int)stage;
-    const int64_t wd = k < kGate ? W : k < kR1 ? (int64_t)N * C : N;
+    const int64_t wd = k < kGate ? W : k < kR1 ? (int64_t)N * C : 4;
     stage += (s->per * wd + 3) & ~3ll;
   }
-  const int64_t fixed = 2 * s->warps * kScratch + (sums && !s->hold ? (2 * N * C + 3) & ~3 : 0);
-  int most = max_warps(mode) / s->warps;
+  const int64_t fixed = 2 * s->warps * kScratch + kBarrierFloats + (sums && !s->hold ? (2 * N * C + 3) & ~3 : 0);
+  int most = max_warps(mode, L) / s->warps;
   if (s->warps > 1 && most > 15) most = 15;      // named barriers
   const int64_t tiles = (rows + s->per - 1) / s->per, wanted = (tiles + sms - 1) / sms;
   if (wanted < most) most = (int)(wanted > 0 ? wanted : 1);
@@ -114,8 +114,15 @@ int run(int mode, BlockArgs& a, int lmax, int layout, bool branch, int* blocks, 
     return ICTC_ERR_UNSUPPORTED;
   }
   a.wide = 0;
+  a.row_bytes = 0;
+  s.bulk = s.hold && s.stages > 1;
   for (int k = 0; k < kSlots; ++k) {
-    const int64_t wd = k < kGate ? (int64_t)C * N * N : k < kR1 ? (int64_t)N * C : N;
+    const int64_t wd = k < kGate ? (int64_t)C * N * N : k < kR1 ? (int64_t)N * C : 4;
+    if (a.in[k]) {
+      a.row_bytes += (int)(4 * wd);
+      if (wd % 4 || !aligned(a.in[k])) s.bulk = 0;
+    }
+    if (k < 6 && a.out[k] && (wd % 4 || !aligned(a.out[k]))) s.bulk = 0;
     if (s.per * wd % 4) continue;
     if (aligned(a.in[k])) a.wide |= 1u << k;
     if (k < 6 && aligned(a.out[k])) a.wide |= 1u << (16 + k);
@@ -179,12 +186,13 @@ extern "C" int ictc_block_supported(int channels, int lmax) {
 extern "C" int ictc_block_forward(const float* stream_in, const float* branch, const float* gate, const float* post,
                                   const float* scale, const float* pre, int norm, int64_t rows, int channels,
                                   int lmax, int layout, float eps, float* stream_out, float* normed, float* r1,
-                                  float* r2, void* stream) {
+                                  float* r2, int* status, void* stream) {
   if (bad_shape(rows, channels, lmax, layout, eps) ||
-      (rows > 0 && (!stream_in || (branch ? !stream_out : !norm) || (norm && !normed))))
+      (rows > 0 && (!stream_in || (branch ? !stream_out : !norm) || (norm && !normed) || !status)))
     return invalid("ictc_block_forward: invalid argument%s");
   if (rows == 0) return ICTC_OK;
   BlockArgs a{};
+  a.status = status;
   a.in[kY] = branch;
   a.in[kH] = stream_in;
   a.out[kY] = norm ? normed : nullptr;      // u leaves from y's place
@@ -206,13 +214,14 @@ extern "C" int ictc_block_backward(const float* stream_out, const float* branch,
                                    const float* scale, const float* pre, const float* r1, const float* r2,
                                    const float* p, const float* q, int64_t rows, int channels, int lmax, int layout,
                                    float* grad_stream, float* grad_branch, float* grad_gate, float* grad_post,
-                                   float* grad_scale, float* grad_pre, float* partial, void* stream) {
+                                   float* grad_scale, float* grad_pre, float* partial, int* status, void* stream) {
   const bool norm = q != nullptr, sums = grad_post || grad_scale || grad_pre;
   if (bad_shape(rows, channels, lmax, layout, 1.f) || (sums && !partial) ||
       (rows > 0 && ((norm && (!stream_out || !r2)) || (branch ? !r1 : !norm) || (!p && !q) ||
-                    (grad_gate && (!gate || !branch)) || (grad_stream && !norm))))
+                    (grad_gate && (!gate || !branch)) || (grad_stream && !norm) || !status)))
     return invalid("ictc_block_backward: invalid argument%s");
   BlockArgs a{};
+  a.status = status;
   a.post = post;
   a.scale = scale;
   a.partial = sums ? partial : nullptr;
@@ -243,13 +252,14 @@ extern "C" int ictc_block_second(const float* stream_out, const float* branch, c
                                  const float* dot_gate, int64_t rows, int channels, int lmax, int layout,
                                  float* grad_stream, float* grad_branch, float* grad_gate, float* grad_post,
                                  float* grad_scale, float* grad_pre, float* grad_p, float* grad_q, float* partial,
-                                 void* stream) {
+                                 int* status, void* stream) {
   const bool norm = q != nullptr, sums = grad_post || grad_scale || grad_pre;
   if (bad_shape(rows, channels, lmax, layout, 1.f) || (sums && !partial) ||
       (rows > 0 && ((norm && (!stream_out || !r2)) || (branch ? !r1 : !norm) || (!p && !q) ||
-                    ((grad_gate || dot_gate) && (!gate || !branch)) || ((grad_stream || grad_q) && !norm))))
+                    ((grad_gate || dot_gate) && (!gate || !branch)) || ((grad_stream || grad_q) && !norm) || !status)))
     return invalid("ictc_block_second: invalid argument%s");
   BlockArgs a{};
+  a.status = status;
   a.post = post;
   a.scale = scale;
   a.partial = sums ? partial : nullptr;

@@ -36,6 +36,7 @@
 
 #include "ictc_common.cuh"
 #include "ictc_cuda.h"
+#include "tc_sm100.cuh"
 
 #include <atomic>
 #include <cstdio>
@@ -57,15 +58,29 @@ enum Mode : int { kForward = 0, kBackward = 1, kSecond = 2 };
 // (without a branch, the norm alone: . h, . h' . q, . h' . q al .)
 enum Slot : int { kY, kH, kP, kQ, kAl, kBe, kGate, kGateDot, kR1, kR2, kSlots };
 
-// Warps per block: what their registers leave room for (85, 128 and 255 of them).
-__host__ __device__ constexpr int max_warps(int mode) { return mode == kForward ? 24 : mode == kBackward ? 16 : 8; }
-// Warps of one row at most (a power of two).
-__host__ __device__ constexpr int max_row_warps(int mode) { return mode == kSecond ? 8 : 16; }
-// Rows that a lane works on at once.
+// Rows that a lane works on at once, and warps per block, by mode and lmax.  Low degrees have few
+// values per row: several rows share a tile's barriers, sums and copies.  More rows per lane mean
+// more registers and so fewer warps; measured on 50,000 to 100,000 rows, both sides of each choice:
+//   forward  lmax 0, C128: 8 rows 74 us, 4 rows 96;  lmax 1, C132: 4 rows 98, 2 rows 127
+//   backward lmax 0, C128: 8 rows 104, 4 rows 141;  lmax 1, C132: 4 rows 223 (16 warps), 2 rows 162 (20 warps);
+//            lmax 2, C64: 2 rows 217, 1 row 178;  lmax 3, 8,192 rows of C128: 16 warps 90, 12 warps 84
+//   second   lmax 0, C128: 4 rows 262 (12 warps), 1 row 315 (16 warps);  lmax 1, C50: 2 rows 133, 1 row 150;
+//            lmax 2, C64: 2 rows 487, 1 row 328
 __host__ __device__ constexpr int rows_per_lane(int mode, int L, bool hold) {
-  return !hold ? 1 : mode == kSecond ? (L == 0 ? 4 : L == 1 ? 2 : 1) : (L == 0 ? 8 : L == 1 ? 4 : L == 2 ? 2 : 1);
+  constexpr int rows[3][kMaxL + 1] = {{8, 4, 2, 1}, {8, 2, 1, 1}, {4, 2, 1, 1}};
+  return hold ? rows[mode][L] : 1;
+}
+__host__ __device__ constexpr int max_warps(int mode, int L) {
+  constexpr int warps[3][kMaxL + 1] = {{24, 24, 20, 20}, {16, 20, 20, 12}, {12, 12, 12, 8}};
+  return warps[mode][L];
+}
+// Warps of one row at most; wider rows take turns (HOLD false).
+__host__ __device__ constexpr int max_row_warps(int mode, int L) {
+  return max_warps(mode, L) < 16 ? max_warps(mode, L) : 16;
 }
 constexpr int kScratch = 16;   // sums of one warp
+constexpr int kBarrierFloats = 8;                     // room of four mbarriers
+constexpr uint64_t kWaitNs = 2000000000ull;           // a copy that takes longer is given up
 
 struct BlockArgs {
   const float* in[kSlots];  // null: zeros, or not there
@@ -76,7 +91,8 @@ struct BlockArgs {
   const float* post;        // [L+1, C] or null (1)
   const float* scale;
   const float* pre;
-  float* r1_out;            // [N, L+1], or null (forward)
+  int* status;              // 1 (3) after a copy did not land in time (nor while draining)
+  float* r1_out;            // [N, 4], or null (forward)
   float* r2_out;
   float* partial;           // [blocks][2][(L+1) C] weight-gradient sums, or null
   int64_t rows;
@@ -87,13 +103,14 @@ struct BlockArgs {
   int stages;
   int stage_floats;
   int group_floats;
+  int row_bytes;            // staged bytes of one row
   int norm;                 // u (or its cotangent) takes part
   float eps;
   float inv[kMaxL + 1];     // 1 / D of every degree
 };
 
 struct Shape {
-  int hold, lanes, warps, per, stages, groups;
+  int hold, bulk, lanes, warps, per, stages, groups;
 };
 
 __device__ __forceinline__ void copy_async16(float* dst, const float* src) {
@@ -122,7 +139,10 @@ struct Group {
 
   __device__ __forceinline__ void sync() const {
     if (threads == 32) __syncwarp();
-    else asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(threads) : "memory");
+    else tc::named_barrier(id + 1, threads);
+  }
+  __device__ __forceinline__ bool sync_all(bool x) const {
+    return threads == 32 ? __all_sync(0xffffffffu, x) : tc::named_barrier_all(id + 1, threads, x);
   }
   // Sums of N values over a row's lanes, in a fixed order, in every lane.  Over whole warps
   // each exchange halves the values that a lane carries on (N - 1 + 5 - log2 N exchanges
@@ -242,8 +262,20 @@ struct Weights {
 #define ICTC_DEGREES(l, N) _Pragma("unroll") for (int l = 0; l < N; ++l)
 #define ICTC_PARTS(e, l) _Pragma("unroll") for (int e = l * l; e < (l + 1) * (l + 1); ++e)
 
-template <int L, int LAYOUT, int MODE, bool BRANCH, bool HOLD>
-__global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __grid_constant__ BlockArgs a) {
+__device__ __forceinline__ void bulk_store(float* dst, const float* src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(tc::smem_u32(src)),
+               "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+// All bulk stores of this thread have read shared memory.
+__device__ __forceinline__ void bulk_read_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+
+// HOLD: a lane has one channel and keeps its values between phases.  BULK: every tensor of a tile is
+// 16-byte aligned and a multiple of 16 bytes and moves by one bulk copy each way, issued by the group's
+// first thread; otherwise all threads copy, 16 or 4 bytes at a time.
+template <int L, int LAYOUT, int MODE, bool BRANCH, bool HOLD, bool BULK>
+__global__ void __launch_bounds__(32 * max_warps(MODE, L)) block_kernel(const __grid_constant__ BlockArgs a) {
   extern __shared__ __align__(16) float shared[];
   constexpr int N = L + 1, R = rows_per_lane(MODE, L, HOLD);
   using V = Vals<R, L>;
@@ -257,7 +289,8 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
   const int groups = blockDim.x / g.threads;
   float* ring = shared + g.id * a.group_floats;
   g.scratch = ring + a.stages * a.stage_floats;
-  float* acc = g.scratch + 2 * a.warps * kScratch;      // weight-gradient sums (HOLD false)
+  uint64_t* full = reinterpret_cast<uint64_t*>(g.scratch + 2 * a.warps * kScratch);      // one per stage
+  float* acc = g.scratch + 2 * a.warps * kScratch + kBarrierFloats;      // weight-gradient sums (HOLD false)
   const int sub = g.thread / a.lanes;                   // this lane's rows are sub + r * (rows / R) of the tile
   const int c0 = g.thread - sub * a.lanes;
   const int apart = a.per / R;
@@ -266,7 +299,25 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
   if (!HOLD && a.partial)
     for (int i = g.thread; i < 2 * width; i += g.threads) acc[i] = 0.f;
 
+  int issued = 0;      // tiles asked for by bulk copies (the group's first thread)
+  // The tile t goes into `stage`; with bulk copies this is the first thread's business alone.
   auto fetch = [&](int64_t t, int stage) {
+    if constexpr (BULK) {
+      if (g.thread == 0 && t < tiles) {
+        const int64_t row0 = t * a.per;
+        const uint32_t rows = (uint32_t)(a.rows - row0 < a.per ? a.rows - row0 : a.per);
+        float* base = ring + stage * a.stage_floats;
+        tc::mbar_arrive_expect(full + stage, rows * a.row_bytes);
+#pragma unroll
+        for (int s = 0; s < kSlots; ++s) {
+          if (a.in[s] == nullptr) continue;
+          const int wd = s < kGate ? W : s < kR1 ? width : 4;
+          tc::bulk_load(base + a.at[s], a.in[s] + row0 * wd, rows * wd * 4, full + stage);
+        }
+        ++issued;
+      }
+      return;
+    }
     if (t < tiles) {
       const int64_t row0 = t * a.per;
       const int rows = (int)(a.rows - row0 < a.per ? a.rows - row0 : a.per);
@@ -274,7 +325,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
 #pragma unroll
       for (int s = 0; s < kSlots; ++s) {
         if (a.in[s] == nullptr || a.at[s] < 0) continue;
-        const int wd = s < kGate ? W : s < kR1 ? width : N;
+        const int wd = s < kGate ? W : s < kR1 ? width : 4;
         float* dst = base + a.at[s];
         const float* src = a.in[s] + row0 * wd;
         const int count = rows * wd;
@@ -303,10 +354,28 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
   ICTC_DEGREES(l, N) sum_w[l] = sum_b[l] = own.w[l] = own.b[l] = 0.f;
   if (HOLD && c0 < C) own.load(a, c0);
 
+  if constexpr (BULK) {
+    if (g.thread == 0)
+      for (int s = 0; s < a.stages; ++s) tc::mbar_init(full + s, 1);
+    g.sync();
+  }
   for (int s = 0; s + 1 < a.stages; ++s) fetch(first + s * stride, s);
-  int stage = 0;
+  int stage = 0, waited = 0;
+  uint32_t parity = 0;
   for (int64_t t = first; t < tiles; t += stride) {
-    if (a.stages == 1) {
+    if constexpr (BULK) {
+      const bool landed = g.sync_all(g.thread != 0 || tc::mbar_wait(full + stage, parity, kWaitNs));
+      if (!landed) {      // report, let the copies in flight end, and leave
+        if (g.thread == 0) {
+          bool drained = true;
+          for (int j = waited; j < issued; ++j)
+            drained = tc::mbar_wait(full + j % a.stages, (j / a.stages) & 1, kWaitNs) && drained;
+          atomicMax(a.status, drained ? 1 : 3);
+        }
+        break;
+      }
+      ++waited;
+    } else if (a.stages == 1) {
       g.sync();
       fetch(t, 0);
       copies_wait(0);
@@ -316,6 +385,15 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
       g.sync();       // the tile is there, and everyone has left the stage that is filled next
       fetch(t + (a.stages - 1) * stride, stage == 0 ? a.stages - 1 : stage - 1);
     }
+    // The stage that the last tile left is filled once its rows have been read out.
+    auto refill = [&]() {
+      if constexpr (BULK) {
+        if (g.thread == 0) {
+          bulk_read_wait();
+          fetch(t + (a.stages - 1) * stride, stage == 0 ? a.stages - 1 : stage - 1);
+        }
+      }
+    };
     float* tile = ring + stage * a.stage_floats;
     const int64_t row0 = t * a.per;
     const int rows = (int)(a.rows - row0 < a.per ? a.rows - row0 : a.per);
@@ -329,6 +407,11 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
     // a value per row, degree and channel (the widest rows leave no room for these)
     auto channel = [&](int s, int r, int l, int c) {
       return HOLD ? tile[a.at[s] + (sub + r * apart) * width + l * C + c] : __ldg(a.in[s] + row0 * width + l * C + c);
+    };
+    // a row's rates, four floats
+    auto keep = [&](float* to, int r, const float* x) {
+      *reinterpret_cast<float4*>(to + (row0 + sub + r * apart) * 4) =
+          make_float4(x[0], N > 1 ? x[1 % N] : 0.f, N > 2 ? x[2 % N] : 0.f, N > 3 ? x[3 % N] : 0.f);
     };
     // sigma(gate) of a channel, per row and degree
     auto sigma = [&](float (&s)[R][N], int c) {
@@ -352,11 +435,12 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
           get(y, kY, c);
           ICTC_ROWS(r, R) ICTC_DEGREES(l, N) ICTC_PARTS(e, l) s[r * N + l] = fmaf(y.v[r][e], y.v[r][e], s[r * N + l]);
         });
+        refill();
         g.sum(s);
         ICTC_ROWS(r, R) ICTC_DEGREES(l, N) r1[r][l] = rate(s[r * N + l], l);
-        if (a.r1_out && c0 == 0)
-          ICTC_ROWS(r, R) if (real[r]) ICTC_DEGREES(l, N)
-            a.r1_out[(row0 + sub + r * apart) * N + l] = r1[r][l];
+        if (a.r1_out && c0 == 0) ICTC_ROWS(r, R) if (real[r]) keep(a.r1_out, r, r1[r]);
+      } else {
+        refill();
       }
       ICTC_ROWS(r, R) ICTC_DEGREES(l, N) s[r * N + l] = 0.f;
       each([&](int c) {
@@ -377,9 +461,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
       if (a.norm) {
         g.sum(s);
         ICTC_ROWS(r, R) ICTC_DEGREES(l, N) s[r * N + l] = rate(s[r * N + l], l);
-        if (a.r2_out && c0 == 0)
-          ICTC_ROWS(r, R) if (real[r]) ICTC_DEGREES(l, N)
-            a.r2_out[(row0 + sub + r * apart) * N + l] = s[r * N + l];
+        if (a.r2_out && c0 == 0) ICTC_ROWS(r, R) if (real[r]) keep(a.r2_out, r, s + r * N);
         each([&](int c) {
           again(h, kH, c);
           weights(c);
@@ -394,7 +476,7 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
       V h, q, T, y;
       float r1[R][N], r2[R][N], kq[R * N];
       ICTC_ROWS(r, R) ICTC_DEGREES(l, N) {
-        const int from = (sub + r * apart) * N + l;
+        const int from = (sub + r * apart) * 4 + l;
         r1[r][l] = BRANCH ? tile[a.at[kR1] + from] : 0.f;
         r2[r][l] = a.norm ? tile[a.at[kR2] + from] : 0.f;
         kq[r * N + l] = 0.f;
@@ -414,9 +496,11 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
             }
           }
         });
+        refill();
         g.sum(kq);
         ICTC_ROWS(r, R) ICTC_DEGREES(l, N) kq[r * N + l] *= a.inv[l];      // <k, b q>
       }
+      if (!a.norm) refill();
       // T = p + r2 (b q - k <k, b q>)
       auto total = [&](int c) {
         if constexpr (BRANCH) {
@@ -606,25 +690,37 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
         }
       }
     }
-    g.sync();
+    // The rows leave (forward: u from y's place).
+    if constexpr (BULK) {
+      tc::fence_async_smem();
+      g.sync();
+      if (g.thread == 0) {
 #pragma unroll
-    for (int s = 0; s < 6; ++s) {
-      // forward: u leaves from y's place
-      if (a.out[s] == nullptr) continue;
-      float* dst = a.out[s] + row0 * W;
-      const float* src = tile + a.at[s];
-      const int count = rows * W;
-      int i = 0;
-      if (a.wide >> (16 + s) & 1u) {
-#pragma unroll 4
-        for (int j = 4 * g.thread; j + 3 < count; j += 4 * g.threads)
-          *reinterpret_cast<float4*>(dst + j) = *reinterpret_cast<const float4*>(src + j);
-        i = count & ~3;
+        for (int s = 0; s < 6; ++s)
+          if (a.out[s]) bulk_store(a.out[s] + row0 * W, tile + a.at[s], rows * W * 4);
+        bulk_commit();
       }
-      for (i += g.thread; i < count; i += g.threads) dst[i] = src[i];
+      if (stage + 1 == a.stages) parity ^= 1;
+    } else {
+      g.sync();
+#pragma unroll
+      for (int s = 0; s < 6; ++s) {
+        if (a.out[s] == nullptr) continue;
+        float* dst = a.out[s] + row0 * W;
+        const float* src = tile + a.at[s];
+        const int count = rows * W;
+        int i = 0;
+        if (a.wide >> (16 + s) & 1u) {
+          for (int j = 4 * g.thread; j + 3 < count; j += 4 * g.threads)
+            *reinterpret_cast<float4*>(dst + j) = *reinterpret_cast<const float4*>(src + j);
+          i = count & ~3;
+        }
+        for (i += g.thread; i < count; i += g.threads) dst[i] = src[i];
+      }
     }
     stage = stage + 1 == a.stages ? 0 : stage + 1;
   }
+  if (BULK && g.thread == 0) bulk_read_wait();      // shared memory outlives the stores that read it
   if (a.partial == nullptr) return;
   // Sums of the block's groups (and of a warp's rows side by side), in order.
   __syncthreads();
@@ -643,15 +739,15 @@ __global__ void __launch_bounds__(32 * max_warps(MODE)) block_kernel(const __gri
       for (int k = 0; k < groups * beside; ++k) s += shared[(int64_t)k * 2 * width + i];
     } else {
       for (int k = 0; k < groups; ++k)
-        s += shared[k * a.group_floats + a.stages * a.stage_floats + 2 * a.warps * kScratch + i];
+        s += shared[k * a.group_floats + a.stages * a.stage_floats + 2 * a.warps * kScratch + kBarrierFloats + i];
     }
     a.partial[(int64_t)blockIdx.x * 2 * width + i] = s;
   }
 }
 
-template <int L, int LAYOUT, int MODE, bool BRANCH, bool HOLD>
+template <int L, int LAYOUT, int MODE, bool BRANCH, bool HOLD, bool BULK>
 cudaError_t launch_one(const BlockArgs& a, const Shape& s, int grid, int shared_bytes, cudaStream_t stream) {
-  auto kernel = block_kernel<L, LAYOUT, MODE, BRANCH, HOLD>;
+  auto kernel = block_kernel<L, LAYOUT, MODE, BRANCH, HOLD, BULK>;
   static std::atomic<bool> ready[kMaxDevices];   // shared-memory limit raised on this device
   int device = 0;
   cudaError_t err = cudaGetDevice(&device);
@@ -665,13 +761,16 @@ cudaError_t launch_one(const BlockArgs& a, const Shape& s, int grid, int shared_
   return cudaGetLastError();
 }
 
+template <int L, int LAYOUT, int MODE, bool BRANCH>
+cudaError_t launch_copies(const BlockArgs& a, const Shape& s, int grid, int bytes, cudaStream_t stream) {
+  if (!s.hold) return launch_one<L, LAYOUT, MODE, BRANCH, false, false>(a, s, grid, bytes, stream);
+  return s.bulk ? launch_one<L, LAYOUT, MODE, BRANCH, true, true>(a, s, grid, bytes, stream)
+                : launch_one<L, LAYOUT, MODE, BRANCH, true, false>(a, s, grid, bytes, stream);
+}
 template <int L, int MODE, bool BRANCH>
 cudaError_t launch_layout(const BlockArgs& a, const Shape& s, int grid, int bytes, int layout, cudaStream_t stream) {
-  if (layout == kMulIr)
-    return s.hold ? launch_one<L, kMulIr, MODE, BRANCH, true>(a, s, grid, bytes, stream)
-                  : launch_one<L, kMulIr, MODE, BRANCH, false>(a, s, grid, bytes, stream);
-  return s.hold ? launch_one<L, kIrMul, MODE, BRANCH, true>(a, s, grid, bytes, stream)
-                : launch_one<L, kIrMul, MODE, BRANCH, false>(a, s, grid, bytes, stream);
+  return layout == kMulIr ? launch_copies<L, kMulIr, MODE, BRANCH>(a, s, grid, bytes, stream)
+                          : launch_copies<L, kIrMul, MODE, BRANCH>(a, s, grid, bytes, stream);
 }
 template <int MODE, bool BRANCH>
 cudaError_t launch_degree(const BlockArgs& a, const Shape& s, int grid, int bytes, int lmax, int layout,

@@ -67,9 +67,9 @@ _SIGNATURES = {
                         _p],
     "ictc_block_partial_floats": [_i, _i],
     "ictc_block_supported": [_i, _i],
-    "ictc_block_forward": [_p] * 6 + [_i, _i64, _i, _i, _i, _f] + [_p] * 5,
-    "ictc_block_backward": [_p] * 10 + [_i64, _i, _i, _i] + [_p] * 8,
-    "ictc_block_second": [_p] * 13 + [_i64, _i, _i, _i] + [_p] * 10,
+    "ictc_block_forward": [_p] * 6 + [_i, _i64, _i, _i, _i, _f] + [_p] * 6,
+    "ictc_block_backward": [_p] * 10 + [_i64, _i, _i, _i] + [_p] * 9,
+    "ictc_block_second": [_p] * 13 + [_i64, _i, _i, _i] + [_p] * 11,
     "ictc_adamw_decode": [_p, _p, _p, _p, _i64, _p, _p, _p],
 }
 _RESTYPES = {"ictc_last_error": ctypes.c_char_p, "ictc_sc_table_rows": _i64,

@@ -93,6 +93,19 @@ def _partial(form, x, wanted):
     return torch.empty(count, device=x.device, dtype=torch.float32)
 
 
+_status = {}
+
+
+def status_word(device):
+    """The device word (int32) that the kernels set when a copy did not land in time."""
+    word = _status.get(device)
+    if word is None:
+        word = torch.zeros(1, dtype=torch.int32, device=device)
+        if not torch.cuda.is_current_stream_capturing():      # a capture's memory is its graph's own
+            _status[device] = word
+    return word
+
+
 def _dense(x):
     return None if x is None else x.contiguous()
 
@@ -102,15 +115,14 @@ class _Block(torch.autograd.Function):
     def forward(ctx, form, stream, branch, gate, post, scale, pre):
         n = stream.shape[0]
         keep = any(ctx.needs_input_grad)
-        width = form.lmax + 1
         out = _like(stream, branch is not None)
         u = _like(stream, form.norm)
-        r1 = torch.empty(n, width, device=stream.device, dtype=torch.float32) if keep and branch is not None else None
-        r2 = torch.empty(n, width, device=stream.device, dtype=torch.float32) if keep and form.norm else None
+        r1 = torch.empty(n, 4, device=stream.device, dtype=torch.float32) if keep and branch is not None else None
+        r2 = torch.empty(n, 4, device=stream.device, dtype=torch.float32) if keep and form.norm else None
         with torch.cuda.device(stream.device):
             _native.call("ictc_block_forward", ptr(stream), ptr(branch), ptr(gate), ptr(post), ptr(scale), ptr(pre),
                          int(form.norm), n, *form.shape, form.eps, ptr(out), ptr(u), ptr(r1), ptr(r2),
-                         stream_of(stream))
+                         ptr(status_word(stream.device)), stream_of(stream))
         ctx.form, ctx.rates = form, (r1, r2)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(stream if out is None else out, branch, gate, post, scale, pre)
@@ -151,7 +163,7 @@ class _BlockGrad(torch.autograd.Function):
             with torch.cuda.device(stream.device):
                 _native.call("ictc_block_backward", ptr(stream), ptr(branch), ptr(gate), ptr(post), ptr(scale),
                              ptr(pre), ptr(r1), ptr(r2), ptr(p), ptr(q), stream.shape[0], *form.shape,
-                             *(ptr(t) for t in out), ptr(partial), stream_of(stream))
+                             *(ptr(t) for t in out), ptr(partial), ptr(status_word(stream.device)), stream_of(stream))
         return tuple(out)
 
     @staticmethod
@@ -187,5 +199,5 @@ class _BlockGrad(torch.autograd.Function):
         with torch.cuda.device(stream.device):
             _native.call("ictc_block_second", ptr(stream), ptr(branch), ptr(gate), ptr(post), ptr(scale), ptr(pre),
                          ptr(r1), ptr(r2), ptr(p), ptr(q), *(ptr(d) for d in dots), stream.shape[0], *form.shape,
-                         *(ptr(t) for t in out), ptr(partial), stream_of(stream))
+                         *(ptr(t) for t in out), ptr(partial), ptr(status_word(stream.device)), stream_of(stream))
         return (None, None, None, *out)

@@ -19,7 +19,8 @@ import torch
 
 from ictc_o3.backends.cuda.runtime import require_cuda_fp32
 
-__all__ = ["degree_norm", "residual_block_norm", "DegreeNorm", "ResidualBlockNorm"]
+__all__ = ["degree_norm", "residual_block_norm", "DegreeNorm", "ResidualBlockNorm",
+           "block_norm_status"]
 
 
 def _form(channels, lmax, layout, eps, norm):
@@ -52,6 +53,18 @@ def _check(form, rows, weights, gate=None):
 
 def _contiguous(x):
     return None if x is None else x.contiguous()
+
+
+def block_norm_status(device="cuda"):
+    """0, or what a kernel of this module left after a copy into shared memory did not land within two
+    seconds (its results are then not valid).  Reads one int from the device: for tests and after a step."""
+    from ictc_o3.backends.cuda.block_norm import status_word
+    device = torch.device(device)
+    if device.type != "cuda":
+        raise ValueError("block norms run on CUDA devices")
+    if device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
+    return int(status_word(device))
 
 
 def degree_norm(features, weight=None, *, channels, lmax, layout="mul_ir", eps=1e-6):

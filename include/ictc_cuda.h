@@ -399,8 +399,11 @@ int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_scale, cons
  *   r(x) = (mean x^2 + eps)^(-1/2)
  *   stream_out = stream + post * scale * sigmoid(gate) * r(branch) * branch
  *   normed     = pre * r(stream_out) * stream_out                 (norm != 0)
- * and with branch = NULL: normed = pre * r(stream) * stream.  r1, r2 [rows, L+1] receive
- * r(branch) and r of the normed rows (NULL: not kept); the derivatives read them.
+ * and with branch = NULL: normed = pre * r(stream) * stream.  r1, r2 [rows, 4]
+ * (16-byte aligned; the first L+1 count) receive r(branch) and r of the normed rows
+ * (NULL: not kept); the derivatives read them.  status: a device int, zeroed by the
+ * caller, that becomes 1 when rows did not arrive in shared memory within two seconds
+ * and the kernel left its work undone (3: the copy may still be in flight).
  *
  * ictc_block_backward: gradients for the cotangents p of stream_out and q of normed
  * (either may be NULL: zero; q = NULL means no norm took part, the gradient of stream
@@ -417,18 +420,19 @@ int64_t ictc_block_partial_floats(int channels, int lmax);
 int ictc_block_supported(int channels, int lmax);
 int ictc_block_forward(const float* stream_in, const float* branch, const float* gate, const float* post,
                        const float* scale, const float* pre, int norm, int64_t rows, int channels, int lmax,
-                       int layout, float eps, float* stream_out, float* normed, float* r1, float* r2, void* stream);
+                       int layout, float eps, float* stream_out, float* normed, float* r1, float* r2, int* status,
+                       void* stream);
 int ictc_block_backward(const float* stream_out, const float* branch, const float* gate, const float* post,
                         const float* scale, const float* pre, const float* r1, const float* r2, const float* p,
                         const float* q, int64_t rows, int channels, int lmax, int layout, float* grad_stream,
                         float* grad_branch, float* grad_gate, float* grad_post, float* grad_scale, float* grad_pre,
-                        float* partial, void* stream);
+                        float* partial, int* status, void* stream);
 int ictc_block_second(const float* stream_out, const float* branch, const float* gate, const float* post,
                       const float* scale, const float* pre, const float* r1, const float* r2, const float* p,
                       const float* q, const float* dot_stream, const float* dot_branch, const float* dot_gate,
                       int64_t rows, int channels, int lmax, int layout, float* grad_stream, float* grad_branch,
                       float* grad_gate, float* grad_post, float* grad_scale, float* grad_pre, float* grad_p,
-                      float* grad_q, float* partial, void* stream);
+                      float* grad_q, float* partial, int* status, void* stream);
 
 #ifdef __cplusplus
 }

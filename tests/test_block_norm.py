@@ -36,26 +36,27 @@ def test_native_entry_points_validate_before_launching():
     some = ctypes.c_void_p(16)
     no = None
 
-    def forward(stream=some, branch=some, norm=1, rows=4, c=8, l=2, layout=1, eps=1e-6, out=some, normed=some):
+    def forward(stream=some, branch=some, norm=1, rows=4, c=8, l=2, layout=1, eps=1e-6, out=some, normed=some,
+                status=some):
         return lib.ictc_block_forward(stream, branch, no, no, no, no, norm, rows, c, l, layout, eps, out, normed, no,
-                                      no, no)
+                                      no, status, no)
 
     for bad in ({"stream": no}, {"out": no}, {"normed": no}, {"rows": -1}, {"c": 0}, {"l": 4}, {"layout": 2},
-                {"eps": 0.0}, {"branch": no, "norm": 0}):
+                {"eps": 0.0}, {"branch": no, "norm": 0}, {"status": no}):
         assert forward(**bad) == -1, bad
         assert "invalid" in lib.ictc_last_error().decode()
     assert forward(rows=0, stream=no, out=no, normed=no) == 0
     assert forward(c=100_000) == -2
     nothing = [no] * 6
     back = lambda p, q, grads, r=some, partial=some: lib.ictc_block_backward(  # noqa: E731
-        some, some, no, no, no, no, r, r, p, q, 4, 8, 2, 1, *grads, partial, no)
+        some, some, no, no, no, no, r, r, p, q, 4, 8, 2, 1, *grads, partial, some, no)
     assert back(no, no, nothing) == -1
     assert back(some, no, [some] + [no] * 5) == -1                # the stream's gradient is p itself
     assert back(some, some, [no] * 3 + [some, no, no], partial=no) == -1
     assert back(some, some, [no, no, some, no, no, no]) == -1     # a gate gradient without a gate
     assert back(some, some, nothing, r=no) == -1
     second = lambda q, dots, grads: lib.ictc_block_second(  # noqa: E731
-        some, some, no, no, no, no, some, some, some, q, *dots, 4, 8, 2, 1, *grads, some, no)
+        some, some, no, no, no, no, some, some, some, q, *dots, 4, 8, 2, 1, *grads, some, some, no)
     assert second(some, [some, some, some], [no] * 8) == -1
     assert second(no, [some, some, no], [no] * 7 + [some]) == -1
     assert lib.ictc_block_partial_floats(8, 4) == -1

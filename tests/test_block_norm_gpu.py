@@ -412,6 +412,10 @@ def test_refusals(cuda_device):
             residual_block_norm(x, bad.pop("branch", x), **form, **bad)
     with pytest.raises(ValueError):
         degree_norm(x[0], w, **form)
+    from ictc_o3.ops.block_norm import block_norm_status
+    assert block_norm_status() == 0
+    with pytest.raises(ValueError):
+        block_norm_status("cpu")
     module = ResidualBlockNorm(8, 2, next_norm=False).to(cuda_device)
     out, none = module(x, x, torch.zeros(4, 3, 8, device=cuda_device))
     assert none is None and out.shape == x.shape
