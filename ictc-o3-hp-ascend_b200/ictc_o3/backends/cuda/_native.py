@@ -128,5 +128,21 @@ def stream_of(tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(tensor.device).cuda_stream)
 
 
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch(device, name, *args):
+    """``call`` with ``device`` current and its current stream as the last argument; tensors may be
+    given for their addresses (None: NULL)."""
+    if torch.cuda.current_device() != device.index:
+        with torch.cuda.device(device):
+            return launch(device, name, *args)
+    stream = torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
+    status = getattr(_lib or library(), name)(
+        *[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args], stream)
+    if status != 0:
+        check(status, name)
+
+
 def call(name, *args):
     check(getattr(library(), name)(*args), name)

@@ -11,7 +11,7 @@ import ctypes
 import torch
 
 from . import _native
-from ._native import ptr, stream_of
+from ._native import launch
 
 BLOCK = 256   # values that share a scale of the 8-bit moments (csrc/adamw.cu)
 
@@ -51,16 +51,14 @@ class TensorTable:
 
     def grad_norm(self, grads, max_norm, skip_nonfinite):
         """``grads``: address of a host array of ``count`` device pointers (0: no gradient)."""
-        _native.call("ictc_adamw_grad_norm", grads, self.count, ptr(self.chunks), self.first_chunk,
-                     1.0 if max_norm is None else max_norm, int(max_norm is not None), int(skip_nonfinite),
-                     ptr(self.workspace), stream_of(self.workspace))
+        launch(self.chunks.device, "ictc_adamw_grad_norm", grads, self.count, self.chunks, self.first_chunk,
+               1.0 if max_norm is None else max_norm, max_norm is not None, skip_nonfinite, self.workspace)
 
     def step(self, weights, grads, first, count, bits, state, *, lr, betas, eps, weight_decay, ema_decay, seed,
              use_norm):
-        _native.call("ictc_adamw_step", weights, grads, first, count, ptr(self.chunks), self.first_chunk, bits,
-                     ptr(state["m"]), ptr(state["v"]), ptr(state["m_scale"]), ptr(state["v_scale"]),
-                     ptr(state["average"]), ptr(state["steps"]), lr, betas[0], betas[1], eps, weight_decay, ema_decay,
-                     seed, int(use_norm), ptr(self.workspace), stream_of(self.workspace))
+        launch(self.chunks.device, "ictc_adamw_step", weights, grads, first, count, self.chunks, self.first_chunk, bits,
+               state["m"], state["v"], state["m_scale"], state["v_scale"], state["average"], state["steps"], lr,
+               betas[0], betas[1], eps, weight_decay, ema_decay, seed, use_norm, self.workspace)
 
     def decode(self, state):
         """BF16 values of the 8-bit moments."""
@@ -68,7 +66,6 @@ class TensorTable:
         m = torch.empty(self.values, dtype=torch.bfloat16, device=device)
         v = torch.empty(self.values, dtype=torch.bfloat16, device=device)
         if self.values:
-            with torch.cuda.device(device):
-                _native.call("ictc_adamw_decode", ptr(state["m"]), ptr(state["v"]), ptr(state["m_scale"]),
-                             ptr(state["v_scale"]), self.values, ptr(m), ptr(v), stream_of(m))
+            launch(device, "ictc_adamw_decode", state["m"], state["v"], state["m_scale"], state["v_scale"],
+                   self.values, m, v)
         return m, v

@@ -11,9 +11,8 @@ from typing import NamedTuple
 
 import torch
 
-from ictc_o3.autograd.adjoint_requirements import required_gradients
 from . import _native
-from ._native import ptr, stream_of
+from ._native import launch
 
 LAYOUTS = {"ir_mul": 0, "mul_ir": 1}
 
@@ -25,10 +24,6 @@ class Form(NamedTuple):
     layout: str
     eps: float
     norm: bool          # normed rows are produced
-
-    @property
-    def shape(self):
-        return self.channels, self.lmax, LAYOUTS[self.layout]
 
 
 def formula(form: Form, stream, branch, gate, post, scale, pre):
@@ -86,10 +81,18 @@ def _like(x, wanted=True):
     return torch.empty_like(x) if wanted and x is not None else None
 
 
+_partial_floats = {}
+
+
 def _partial(form, x, wanted):
+    """Scratch of the weight gradients' sums."""
     if not wanted:
         return None
-    count = int(_native.library().ictc_block_partial_floats(form.channels, form.lmax))
+    key = (x.device, form.channels, form.lmax)
+    count = _partial_floats.get(key)
+    if count is None:
+        with torch.cuda.device(x.device):
+            count = _partial_floats[key] = int(_native.library().ictc_block_partial_floats(form.channels, form.lmax))
     return torch.empty(count, device=x.device, dtype=torch.float32)
 
 
@@ -110,20 +113,49 @@ def _dense(x):
     return None if x is None else x.contiguous()
 
 
+def _forward(form, keep, stream, branch, gate, post, scale, pre):
+    """(stream', normed, r1, r2): what is not produced, or without ``keep`` not kept, is None."""
+    n, device = stream.shape[0], stream.device
+    out = None if branch is None else torch.empty_like(stream)
+    u = torch.empty_like(stream) if form.norm else None
+    r1 = torch.empty(n, 4, device=device, dtype=torch.float32) if keep and branch is not None else None
+    r2 = torch.empty(n, 4, device=device, dtype=torch.float32) if keep and form.norm else None
+    launch(device, "ictc_block_forward", stream, branch, gate, post, scale, pre, form.norm, n, form.channels, form.lmax,
+           LAYOUTS[form.layout], form.eps, out, u, r1, r2, status_word(device))
+    return out, u, r1, r2
+
+
+def _first(form, rates, need, stream, branch, gate, post, scale, pre, p, q):
+    """Gradients of (stream, branch, gate, post, scale, pre), None where ``need`` is false."""
+    out = [_like(t, w) for t, w in zip((stream, branch, gate, post, scale, pre), need)]
+    if q is None:
+        out[0] = out[5] = None
+    if any(t is not None for t in out):
+        partial = _partial(form, stream, any(t is not None for t in out[3:]))
+        launch(stream.device, "ictc_block_backward", stream, branch, gate, post, scale, pre, *rates, p, q,
+               stream.shape[0], form.channels, form.lmax, LAYOUTS[form.layout], *out, partial,
+               status_word(stream.device))
+    return tuple(out)
+
+
+_probe = getattr(torch._C, "_will_engine_execute_node", None)
+
+
+def _runs(node):
+    """Whether the running backward pass executes an input's gradient node (true where it cannot tell)."""
+    if _probe is None or node is None or hasattr(node, "variable"):      # a leaf: the engine does not say
+        return True
+    try:
+        return _probe(node)
+    except RuntimeError:
+        return True
+
+
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, form, stream, branch, gate, post, scale, pre):
-        n = stream.shape[0]
-        keep = any(ctx.needs_input_grad)
-        out = _like(stream, branch is not None)
-        u = _like(stream, form.norm)
-        r1 = torch.empty(n, 4, device=stream.device, dtype=torch.float32) if keep and branch is not None else None
-        r2 = torch.empty(n, 4, device=stream.device, dtype=torch.float32) if keep and form.norm else None
-        with torch.cuda.device(stream.device):
-            _native.call("ictc_block_forward", ptr(stream), ptr(branch), ptr(gate), ptr(post), ptr(scale), ptr(pre),
-                         int(form.norm), n, *form.shape, form.eps, ptr(out), ptr(u), ptr(r1), ptr(r2),
-                         ptr(status_word(stream.device)), stream_of(stream))
-        ctx.form, ctx.rates = form, (r1, r2)
+        out, u, *ctx.rates = _forward(form, True, stream, branch, gate, post, scale, pre)
+        ctx.form = form
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(stream if out is None else out, branch, gate, post, scale, pre)
         return (u,) if out is None else (out,) if u is None else (out, u)
@@ -136,14 +168,18 @@ class _Block(torch.autograd.Function):
         q = cotangents[-1] if form.norm else None
         if p is None and q is None:
             return (None,) * 7
-        need = required_gradients((None, stream, branch, gate, post, scale, pre),
-                                  (False, *ctx.needs_input_grad[1:]))
-        # the saved stream is this operator's output: whether the input's gradient runs is declared
-        need = (False, ctx.needs_input_grad[1], *need[2:])
-        grads = _BlockGrad.apply(form, ctx.rates, need[1:], stream, branch, gate, post, scale, pre, _dense(p),
-                                 _dense(q))
+        # asked of the engine: whether the branch's gradient runs (a row written or not) and whether any
+        # weight's does (forces need none); the weights share their sums, and a gate's gradient is small
+        _, need_stream, need_branch, need_gate, *need_weights = ctx.needs_input_grad
+        nodes = iter([node for node, _ in ctx.next_functions])      # of the tensors among the arguments
+        _, at_branch, _, *at_weights = [None if t is None else next(nodes) for t in ctx.saved_tensors]
+        need_branch = need_branch and _runs(at_branch)
+        runs = any(n and _runs(node) for n, node in zip(need_weights, at_weights))
+        need = (need_stream, need_branch, need_gate, *[n and runs for n in need_weights])
+        args = (form, ctx.rates, need, stream, branch, gate, post, scale, pre, _dense(p), _dense(q))
+        grads = _BlockGrad.apply(*args) if torch.is_grad_enabled() else _first(*args)
         dx = p if q is None else grads[0]
-        return (None, dx if need[1] else None, *grads[1:])
+        return (None, dx if need[0] else None, *grads[1:])
 
 
 class _BlockGrad(torch.autograd.Function):
@@ -154,21 +190,11 @@ class _BlockGrad(torch.autograd.Function):
         ctx.form, ctx.rates = form, rates
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(stream, branch, gate, post, scale, pre, p, q)
-        r1, r2 = rates
-        out = [_like(t, w) for t, w in zip((stream, branch, gate, post, scale, pre), need)]
-        if q is None:
-            out[0] = out[5] = None
-        if branch is not None or out[0] is not None or out[5] is not None:
-            partial = _partial(form, stream, any(w is not None for w in out[3:]))
-            with torch.cuda.device(stream.device):
-                _native.call("ictc_block_backward", ptr(stream), ptr(branch), ptr(gate), ptr(post), ptr(scale),
-                             ptr(pre), ptr(r1), ptr(r2), ptr(p), ptr(q), stream.shape[0], *form.shape,
-                             *(ptr(t) for t in out), ptr(partial), ptr(status_word(stream.device)), stream_of(stream))
-        return tuple(out)
+        return _first(form, rates, need, stream, branch, gate, post, scale, pre, p, q)
 
     @staticmethod
     def backward(ctx, dot_stream, dot_branch, dot_gate, *dot_weights):
-        form, (r1, r2) = ctx.form, ctx.rates
+        form = ctx.form
         saved = ctx.saved_tensors
         stream, branch, gate, post, scale, pre, p, q = saved
         need = ctx.needs_input_grad[3:]
@@ -194,10 +220,20 @@ class _BlockGrad(torch.autograd.Function):
         out = [_like(t, w) for t, w in zip(saved, need)]
         if q is None:
             out[0] = out[5] = out[7] = None
-        partial = _partial(form, stream, any(w is not None for w in out[3:6]))
-        dots = [_dense(d) for d in dots[:3]]
-        with torch.cuda.device(stream.device):
-            _native.call("ictc_block_second", ptr(stream), ptr(branch), ptr(gate), ptr(post), ptr(scale), ptr(pre),
-                         ptr(r1), ptr(r2), ptr(p), ptr(q), *(ptr(d) for d in dots), stream.shape[0], *form.shape,
-                         *(ptr(t) for t in out), ptr(partial), ptr(status_word(stream.device)), stream_of(stream))
+        partial = _partial(form, stream, any(t is not None for t in out[3:6]))
+        launch(stream.device, "ictc_block_second", stream, branch, gate, post, scale, pre, *ctx.rates, p, q,
+               *[_dense(d) for d in dots[:3]], stream.shape[0], form.channels, form.lmax, LAYOUTS[form.layout], *out,
+               partial, status_word(stream.device))
         return (None, None, None, *out)
+
+
+def block(form, stream, branch, gate, post, scale, pre):
+    """(stream', normed) of contiguous arguments; without anything to differentiate no graph is made."""
+    args = (stream, branch, gate, post, scale, pre)
+    if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args]):
+        # views of leaves: a pass for forces can tell that their gradients do not run
+        post, scale, pre = [w.view_as(w) if w is not None and w.requires_grad and w.is_leaf else w
+                            for w in (post, scale, pre)]
+        out = _Block.apply(form, stream, branch, gate, post, scale, pre)
+        return (None, out[0]) if branch is None else out if form.norm else (out[0], None)
+    return _forward(form, False, *args)[:2]

@@ -15,17 +15,20 @@ need both); higher ones go through torch operations.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
+from ictc_o3.backends.cuda import _native
+from ictc_o3.backends.cuda.block_norm import LAYOUTS, Form, block, status_word
 from ictc_o3.backends.cuda.runtime import require_cuda_fp32
 
 __all__ = ["degree_norm", "residual_block_norm", "DegreeNorm", "ResidualBlockNorm",
            "block_norm_status"]
 
 
+@functools.lru_cache(maxsize=256, typed=True)
 def _form(channels, lmax, layout, eps, norm):
-    from ictc_o3.backends.cuda import _native
-    from ictc_o3.backends.cuda.block_norm import LAYOUTS, Form
     if not isinstance(channels, int) or isinstance(channels, bool) or channels < 1:
         raise ValueError("channels must be a positive integer")
     if not isinstance(lmax, int) or isinstance(lmax, bool) or not 0 <= lmax <= 3:
@@ -40,25 +43,24 @@ def _form(channels, lmax, layout, eps, norm):
 
 
 def _check(form, rows, weights, gate=None):
-    n, c, width = rows[0].shape[0], form.channels, form.channels * (form.lmax + 1) ** 2
-    given = [w for w in weights if w is not None]
-    require_cuda_fp32(*rows, *given, *([] if gate is None else [gate]))
-    if any(x.ndim != 2 or x.shape != (n, width) for x in rows):
+    c, degrees = form.channels, form.lmax + 1
+    n = rows[0].shape[0] if rows[0].ndim else 0
+    require_cuda_fp32(*rows, *weights, *(() if gate is None else (gate,)))
+    if any(x.shape != (n, c * degrees * degrees) for x in rows):
         raise ValueError("Rows must have shape [N,C*(L+1)^2]")
-    if any(w.shape != (form.lmax + 1, c) for w in given):
+    if any(w.shape != (degrees, c) for w in weights):
         raise ValueError("Weights must have shape [L+1,C]")
-    if gate is not None and gate.shape not in ((n, (form.lmax + 1) * c), (n, form.lmax + 1, c)):
+    if gate is not None and gate.shape != (n, degrees * c) and gate.shape != (n, degrees, c):
         raise ValueError("Gates must have shape [N,(L+1)*C] or [N,L+1,C]")
 
 
 def _contiguous(x):
-    return None if x is None else x.contiguous()
+    return x if x is None or x.is_contiguous() else x.contiguous()
 
 
 def block_norm_status(device="cuda"):
     """0, or what a kernel of this module left after a copy into shared memory did not land within two
     seconds (its results are then not valid).  Reads one int from the device: for tests and after a step."""
-    from ictc_o3.backends.cuda.block_norm import status_word
     device = torch.device(device)
     if device.type != "cuda":
         raise ValueError("block norms run on CUDA devices")
@@ -69,10 +71,9 @@ def block_norm_status(device="cuda"):
 
 def degree_norm(features, weight=None, *, channels, lmax, layout="mul_ir", eps=1e-6):
     """weight * r(features) * features: the norm before the first block."""
-    from ictc_o3.backends.cuda.block_norm import _Block
     form = _form(channels, lmax, layout, eps, True)
-    _check(form, [features], [weight])
-    return _Block.apply(form, features.contiguous(), None, None, None, None, _contiguous(weight))[0]
+    _check(form, (features,), () if weight is None else (weight,))
+    return block(form, _contiguous(features), None, None, None, None, _contiguous(weight))[1]
 
 
 def residual_block_norm(stream, branch, *, channels, lmax, post_weight=None, scale=None, gate=None, pre_weight=None,
@@ -81,18 +82,16 @@ def residual_block_norm(stream, branch, *, channels, lmax, post_weight=None, sca
 
     Weights [L+1, C] (None: ones), gate [N, (L+1) C] before its sigmoid (None: no gate).  ``norm``:
     whether the normed rows are wanted (default: when ``pre_weight`` is given); normed is None without."""
-    from ictc_o3.backends.cuda.block_norm import _Block
     if norm is None:
         norm = pre_weight is not None
     if not isinstance(norm, bool) or (pre_weight is not None and not norm):
         raise ValueError("norm must be a boolean, and true where pre_weight is given")
     form = _form(channels, lmax, layout, eps, norm)
-    _check(form, [stream, branch], [post_weight, scale, pre_weight], gate)
-    if gate is not None:
-        gate = gate.reshape(gate.shape[0], (lmax + 1) * channels).contiguous()
-    out = _Block.apply(form, stream.contiguous(), branch.contiguous(), gate, _contiguous(post_weight),
-                       _contiguous(scale), _contiguous(pre_weight))
-    return out if norm else (out[0], None)
+    _check(form, (stream, branch), tuple(w for w in (post_weight, scale, pre_weight) if w is not None), gate)
+    if gate is not None and gate.ndim == 3:
+        gate = gate.reshape(gate.shape[0], (lmax + 1) * channels)
+    return block(form, _contiguous(stream), _contiguous(branch), _contiguous(gate), _contiguous(post_weight),
+                 _contiguous(scale), _contiguous(pre_weight))
 
 
 class DegreeNorm(torch.nn.Module):

@@ -118,7 +118,9 @@ class AdamW(torch.optim.Optimizer):
                     entry["ema"] = flat["average"][place].view(p.shape)
                     entry["ema"].copy_(p.detach())
                 self.state[p] = entry
-        self._params, self._sizes, self._flat, self._device = params, [p.numel() for p in params], flat, device
+        self._params, self._flat, self._device = params, flat, device
+        self._expected = [(torch.float32, device.index, p.numel(), True) for p in params]
+        self._full = all(p.numel() for p in params)
         self._table = table
         self._empty = table.workspace.data_ptr()      # stands for the gradient of a tensor without values
 
@@ -130,25 +132,27 @@ class AdamW(torch.optim.Optimizer):
     def _gather(self):
         """Addresses of weights and gradients (0: no gradient), the updated weights, and
         temporaries that must outlive the launch."""
-        weights, grads, live, kept = [], [], [], []
-        device, fp32, strided = self._device, torch.float32, torch.strided
-        for p, size in zip(self._params, self._sizes):
-            g = p.grad
-            if g is None:
-                weights.append(0)
-                grads.append(0)
-                continue
-            if p.dtype is not fp32 or p.device != device or p.numel() != size or not p.is_contiguous():
-                raise ValueError("a parameter has changed its type, device, size or layout since the optimizer was built")
-            if g.dtype is not fp32 or g.layout is not strided or g.device != device or g.numel() != size:
-                raise ValueError("gradients must be dense CUDA FP32 tensors of their parameter's size")
-            if not g.is_contiguous():
-                g = g.contiguous()
-                kept.append(g)
-            weights.append(p.data_ptr())
-            grads.append(g.data_ptr() if size else self._empty)
-            live.append(p)
-        return array("Q", weights), array("Q", grads), live, kept
+        params = self._params
+        grads = [p.grad for p in params]
+        live, expected, given, kept = params, self._expected, grads, ()
+        if any([g is None for g in grads]):
+            live = [p for p, g in zip(params, grads) if g is not None]
+            expected = [e for e, g in zip(self._expected, grads) if g is not None]
+            given = [g for g in grads if g is not None]
+        # one comparison of all at once; what differs is looked at below
+        if [(p.dtype, p.get_device(), p.numel(), p.is_contiguous()) for p in live] != expected:
+            raise ValueError("a parameter has changed its type, device, size or layout since the optimizer was built")
+        if any([g.is_sparse for g in given]) or (
+                [(g.dtype, g.get_device(), g.numel(), g.is_contiguous()) for g in given] != expected):
+            for g, e in zip(given, expected):
+                if g.layout is not torch.strided or (g.dtype, g.get_device(), g.numel()) != e[:3]:
+                    raise ValueError("gradients must be dense CUDA FP32 tensors of their parameter's size")
+            grads = kept = [None if g is None else g.detach().contiguous() for g in grads]
+        if live is params and self._full:
+            return array("Q", [p.data_ptr() for p in params]), array("Q", [g.data_ptr() for g in grads]), live, kept
+        # a tensor without values has no address, but its steps count
+        return (array("Q", [p.data_ptr() for p in params]),
+                array("Q", [0 if g is None else g.data_ptr() or self._empty for g in grads]), live, kept)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -157,21 +161,21 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         groups = [_hyperparameters(group) for group in self.param_groups]
-        with torch.cuda.device(self._device):
-            weights, grads, live, kept = self._gather()
-            if not live:
-                return loss
-            w, g = weights.buffer_info()[0], grads.buffer_info()[0]
-            use_norm = self.max_norm is not None or self.skip_nonfinite
-            if use_norm:
-                self._table.grad_norm(g, self.max_norm, self.skip_nonfinite)
-            first = 0
-            for group, values in zip(self.param_groups, groups):
-                count = len(group["params"])
-                self._table.step(w, g, first, count, self.state_bits, self._flat, **values,
-                                 ema_decay=0.0 if self.ema_decay is None else self.ema_decay, seed=self.seed,
-                                 use_norm=use_norm)
-                first += count
+        weights, grads, live, kept = self._gather()
+        if not live:
+            return loss
+        w, g = weights.buffer_info()[0], grads.buffer_info()[0]
+        use_norm = self.max_norm is not None or self.skip_nonfinite
+        if use_norm:
+            self._table.grad_norm(g, self.max_norm, self.skip_nonfinite)
+        first = 0
+        for group, values in zip(self.param_groups, groups):
+            count = len(group["params"])
+            self._table.step(w, g, first, count, self.state_bits, self._flat, **values,
+                             ema_decay=0.0 if self.ema_decay is None else self.ema_decay, seed=self.seed,
+                             use_norm=use_norm)
+            first += count
+        del kept                     # copies of gradients: their memory is reused on this stream only
         torch.autograd.graph.increment_version(live)
         return loss
 
