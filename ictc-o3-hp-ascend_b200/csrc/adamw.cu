@@ -43,9 +43,24 @@ constexpr int kChunk = 2048;          // values per block: 8 per thread
 constexpr int kQuads = 2;             // groups of 4 values per thread
 constexpr int kBlockValues = 256;     // values that share a scale: 32 lanes x 8
 constexpr int kNormBlocks = 1184;     // partial sums of the gradient norm at most
+constexpr int kRounds = 7;            // of Philox: the fewest its authors report as passing their tests
 constexpr int kList = 240;            // tensors per launch: 16 B each, below 4 KB of parameters
 
 static_assert(kChunk == kThreads * kQuads * 4 && kBlockValues == 32 * kQuads * 4, "a warp owns one scale block");
+
+// A tensor's bias corrections for its next step, left behind by the last one: a block then reads
+// them with its values instead of waiting for one thread's FP64 exponentials (8-bit states, 160 M
+// values: 820 -> 716 us).  They hold for the step number and betas they name, else they are made again.
+struct alignas(32) Rate {
+  float m;        // 1 / (1 - b1^t)
+  float v;        // 1 / sqrt(1 - b2^t)
+  float b1, b2;
+  int64_t t;
+};
+
+__device__ __forceinline__ Rate rate_of(int64_t t, double log_b1, double log_b2, float b1, float b2) {
+  return Rate{(float)(1.0 / -expm1((double)t * log_b1)), (float)(1.0 / sqrt(-expm1((double)t * log_b2))), b1, b2, t};
+}
 
 // Caller-owned device words, zeroed once.  The tickets count finished blocks and return
 // to zero at the end of each launch.
@@ -80,12 +95,13 @@ struct Args {
   uint8_t* v_scale;
   float* average;
   int64_t* steps;
+  Rate* rates;
   Workspace* ws;
   int use_norm;
   float b1, c1, b2, c2;      // betas and 1 - beta
-  float eps, keep, avg, avg1;  // keep = 1 - lr wd
-  double lr, log_b1, log_b2;
-  uint32_t seed_lo, seed_hi;
+  float lr, eps, keep, avg, avg1;  // keep = 1 - lr wd
+  double log_b1, log_b2;
+  uint2 keys[kRounds];       // Philox key schedule of the seed
 };
 
 __device__ __forceinline__ float4 load4(const float* p, int left, bool aligned) {
@@ -110,39 +126,64 @@ __device__ __forceinline__ void store4(float* p, const float (&x)[4], int left, 
 
 __device__ __forceinline__ bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-// Seven rounds of Philox4x32 (the fewest its authors report as passing their tests).
-__device__ __forceinline__ uint4 philox7(uint4 c, uint32_t k0, uint32_t k1) {
+// Philox4x32 with the keys of its rounds given.
+__device__ __forceinline__ uint4 philox(uint4 c, const uint2 (&keys)[kRounds]) {
 #pragma unroll
-  for (int r = 0; r < 7; ++r) {
+  for (int r = 0; r < kRounds; ++r) {
     const uint64_t a = (uint64_t)c.x * 0xD2511F53u;
     const uint64_t b = (uint64_t)c.z * 0xCD9E8D57u;
-    c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ k0, (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ k1, (uint32_t)a);
-    k0 += 0x9E3779B9u;
-    k1 += 0xBB67AE85u;
+    c = make_uint4((uint32_t)(b >> 32) ^ c.y ^ keys[r].x, (uint32_t)b, (uint32_t)(a >> 32) ^ c.w ^ keys[r].y,
+                   (uint32_t)a);
   }
   return c;
 }
 
+// Value of the code in byte i of a word.
 template <bool SIGNED>
-__device__ __forceinline__ float decode(uint32_t code, float scale) {
-  const uint32_t low = SIGNED ? code & 127u : code;
-  const float x = low ? __uint_as_float((low + (SIGNED ? 896u : 768u)) << 20) * scale : 0.f;
-  return SIGNED && (code & 128u) ? -x : x;
+__device__ __forceinline__ float decode(uint32_t word, int i, float scale) {
+  const uint32_t top = __byte_perm(word, 0, i << 12 | 0x0444);      // the byte in bits 24..31, zeros below
+  const uint32_t low = SIGNED ? top >> 4 & 0x07f00000u : top >> 4;
+  uint32_t bits = low + ((SIGNED ? 896u : 768u) << 20);
+  if (SIGNED) bits |= top & 0x80000000u;
+  return low ? __uint_as_float(bits) * scale : 0.f;
 }
 
+// Codes of four values in a word, r16: random bits in each's lowest 16 (a's own half of the
+// Philox words).  As a rule all magnitudes lie between the least code's value and the block's
+// largest, and a code is the top of the pattern plus random bits below it: 896 and 768 are multiples of
+// a code's range, so the low bits of the sum need no subtraction.  `rare` covers the rest: zeros and
+// values below the least code, or scales at their limit.
 template <bool SIGNED>
-__device__ __forceinline__ uint32_t encode(float x, float inv_scale, uint32_t r16) {
-  constexpr int base = SIGNED ? 896 : 768;
+__device__ __forceinline__ uint32_t encode(const float (&x)[4], float inv_scale, const uint32_t (&r)[4], bool top) {
   constexpr float least = SIGNED ? 1.125f / 32768.f : 1.125f / 2147483648.f;
-  const float a = fabsf(x) * inv_scale;
-  uint32_t code;
-  if (a < least) {
-    code = SIGNED ? ((float)r16 < a * (65536.f / least) ? 1u : 0u) : (a > 0.f ? 1u : 0u);
-  } else {
-    code = ((__float_as_uint(a) + (r16 << 4)) >> 20) - base;
-    code = min(code, SIGNED ? 127u : 255u);
+  float a[4];
+  uint32_t q[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    a[i] = fabsf(x[i]) * inv_scale;
+    const uint32_t r16 = SIGNED ? r[i] & 0xffffu : r[i] >> 16;
+    q[i] = (__float_as_uint(a[i]) + (r16 << 4)) >> 20;
   }
-  return SIGNED && x < 0.f && code ? code | 128u : code;
+  const bool rare = top || fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) < least;
+  if (rare) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t r16 = SIGNED ? r[i] & 0xffffu : r[i] >> 16;
+      if (a[i] < least) q[i] = SIGNED ? ((float)r16 < a[i] * (65536.f / least) ? 1u : 0u) : (a[i] > 0.f ? 1u : 0u);
+      else q[i] = min(q[i] - (SIGNED ? 896u : 768u), SIGNED ? 127u : 255u);
+    }
+  }
+  const uint32_t codes = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+  if (!SIGNED) return codes;
+  const uint32_t signs = __byte_perm(__byte_perm(__float_as_uint(x[0]), __float_as_uint(x[1]), 0x0073),
+                                     __byte_perm(__float_as_uint(x[2]), __float_as_uint(x[3]), 0x0073), 0x5410);
+  uint32_t out = (codes & 0x7f7f7f7fu) | (signs & 0x80808080u);
+  if (rare) {      // no sign without a value
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (q[i] == 0) out &= ~(0xffu << (8 * i));
+  }
+  return out;
 }
 
 // Exponent byte of a block from its largest magnitude's bits.
@@ -171,22 +212,37 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
                                                              int clip, int skip_bad) {
   __shared__ double shared[kThreads / 32];
   __shared__ int last;
+  constexpr int kAhead = 4;      // chunks whose values are in flight together
   double sum = 0.0;
-  for (int64_t i = blockIdx.x; i < a.chunks_n; i += gridDim.x) {
-    const int4 c = a.chunks[a.chunk0 + i];
-    const float* g = list.t[c.x - a.tensor0].grad;
-    if (g == nullptr) continue;
-    g += (int64_t)c.w * kChunk;
-    const bool al = aligned16(g);
+  for (int64_t i0 = blockIdx.x; i0 < a.chunks_n; i0 += kAhead * (int64_t)gridDim.x) {
+    int4 c[kAhead];
+    float4 x[kAhead][kQuads];
 #pragma unroll
-    for (int q = 0; q < kQuads; ++q) {
-      const int at = (q * kThreads + threadIdx.x) * 4;
-      const float4 x = load4(g + at, c.y - at, al);
-      sum += (double)x.x * x.x;
-      sum += (double)x.y * x.y;
-      sum += (double)x.z * x.z;
-      sum += (double)x.w * x.w;
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = i0 + k * (int64_t)gridDim.x;
+      c[k] = i < a.chunks_n ? a.chunks[a.chunk0 + i] : make_int4(a.tensor0, 0, 0, 0);
     }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const float* g = list.t[c[k].x - a.tensor0].grad;
+      if (g == nullptr) c[k].y = 0;
+      g += (int64_t)c[k].w * kChunk;
+      const bool al = aligned16(g);
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) {
+        const int at = (q * kThreads + threadIdx.x) * 4;
+        x[k][q] = load4(g + at, c[k].y - at, al);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+#pragma unroll
+      for (int q = 0; q < kQuads; ++q) {
+        sum += (double)x[k][q].x * x[k][q].x;
+        sum += (double)x[k][q].y * x[k][q].y;
+        sum += (double)x[k][q].z * x[k][q].z;
+        sum += (double)x[k][q].w * x[k][q].w;
+      }
   }
   sum = block_sum(sum, shared);
   if (threadIdx.x == 0) {
@@ -214,21 +270,15 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
 }
 
 template <int BITS, bool AVERAGE>
-__global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
-  __shared__ float s_size, s_rate;
-  __shared__ int64_t s_t;
+__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
   __shared__ int s_last;
   const int4 c = a.chunks_n ? a.chunks[a.chunk0 + blockIdx.x] : make_int4(a.tensor0, 0, 0, 0);
   const Tensor tensor = list.t[c.x - a.tensor0];
   const bool skip = a.use_norm && a.ws->skip;
   const bool active = tensor.grad != nullptr && !skip;
   if (active) {
-    if (threadIdx.x == 0) {
-      const int64_t t = a.steps[c.x] + 1;
-      s_t = t;
-      s_size = (float)(a.lr / -expm1((double)t * a.log_b1));
-      s_rate = (float)(1.0 / sqrt(-expm1((double)t * a.log_b2)));
-    }
+    const int64_t t = a.steps[c.x] + 1;
+    Rate rate = a.rates[c.x];
     float clip = 1.f;
     if (a.use_norm) clip = a.ws->clip;
     float* wp = tensor.weight + (int64_t)c.w * kChunk;
@@ -262,47 +312,54 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
           const uint32_t vc = *reinterpret_cast<const uint32_t*>((const uint8_t*)a.v + s0 + q * 128);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            m[q][i] = decode<true>((mc >> (8 * i)) & 255u, ms);
-            v[q][i] = decode<false>((vc >> (8 * i)) & 255u, vs);
+            m[q][i] = decode<true>(mc, i, ms);
+            v[q][i] = decode<false>(vc, i, vs);
           }
         }
       }
     }
-    __syncthreads();
     if (used) {
-      const float size = s_size, rate = s_rate;
-      float mmax = 0.f, vmax = 0.f;
-      bool fine = true;
+      if (rate.t != t || rate.b1 != a.b1 || rate.b2 != a.b2) rate = rate_of(t, a.log_b1, a.log_b2, a.b1, a.b2);
+      const float size = a.lr * rate.m;
+      uint32_t mmax = 0, vmax = 0;      // as patterns: infinities and NaN are the largest
 #pragma unroll
       for (int q = 0; q < kQuads; ++q) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float x = a.use_norm ? __fmul_rn(g[q][i], clip) : g[q][i];
+          const float x = __fmul_rn(g[q][i], clip);
           m[q][i] = __fadd_rn(__fmul_rn(m[q][i], a.b1), __fmul_rn(x, a.c1));
           v[q][i] = __fadd_rn(__fmul_rn(v[q][i], a.b2), __fmul_rn(__fmul_rn(x, x), a.c2));
           if constexpr (BITS == 8) {
-            fine = fine && isfinite(m[q][i]) && isfinite(v[q][i]);
-            mmax = fmaxf(mmax, fabsf(m[q][i]));
-            vmax = fmaxf(vmax, v[q][i]);
+            mmax = max(mmax, __float_as_uint(fabsf(m[q][i])));
+            vmax = max(vmax, __float_as_uint(v[q][i]));      // a NaN of a sum of squares is positive
+            // bound by its instructions: hardware root and quotient (within 2 units in the last place)
+            float root;
+            asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v[q][i]));
+            const float den = fmaf(root, rate.v, a.eps);
+            w[q][i] = fmaf(w[q][i], a.keep, -size * __fdividef(m[q][i], den));
+          } else {
+            const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v[q][i]), rate.v), a.eps);
+            w[q][i] = __fsub_rn(__fmul_rn(w[q][i], a.keep), __fmul_rn(size, __fdiv_rn(m[q][i], den)));
           }
-          const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v[q][i]), rate), a.eps);
-          w[q][i] = __fsub_rn(__fmul_rn(w[q][i], a.keep), __fmul_rn(size, __fdiv_rn(m[q][i], den)));
         }
       }
-      bool write = true;
-      if constexpr (BITS == 8) write = __all_sync(0xffffffffu, fine);
-      if (write) {
-        float mi = 0.f, vi = 0.f;
-        if constexpr (BITS == 8) {
-          const uint32_t mb = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(mmax)));
-          const uint32_t vb = scale_byte(__reduce_max_sync(0xffffffffu, __float_as_uint(vmax)));
-          mi = __uint_as_float((254u - mb) << 23);
-          vi = __uint_as_float((254u - vb) << 23);
-          if (lane == 0) {
-            a.m_scale[block] = (uint8_t)mb;
-            a.v_scale[block] = (uint8_t)vb;
-          }
+      bool write = true, mtop = false, vtop = false;
+      float mi = 0.f, vi = 0.f;
+      if constexpr (BITS == 8) {
+        mmax = __reduce_max_sync(0xffffffffu, mmax);
+        vmax = __reduce_max_sync(0xffffffffu, vmax);
+        write = max(mmax, vmax) < 0x7f800000u;
+        const uint32_t mb = scale_byte(mmax), vb = scale_byte(vmax);
+        mtop = mb == 253u;
+        vtop = vb == 253u;
+        mi = __uint_as_float((254u - mb) << 23);
+        vi = __uint_as_float((254u - vb) << 23);
+        if (write && lane == 0) {
+          a.m_scale[block] = (uint8_t)mb;
+          a.v_scale[block] = (uint8_t)vb;
         }
+      }
+      if (write) {
 #pragma unroll
         for (int q = 0; q < kQuads; ++q) {
           const int at = at0 + q * 128;
@@ -312,16 +369,10 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
             *reinterpret_cast<float4*>((float*)a.v + s0 + q * 128) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
           } else {
             const uint64_t quad = (uint64_t)(s0 + q * 128) >> 2;
-            const uint64_t t = (uint64_t)s_t;
-            const uint4 r = philox7(make_uint4((uint32_t)quad, (uint32_t)(quad >> 32), (uint32_t)t,
-                                               (uint32_t)(t >> 32)), a.seed_lo, a.seed_hi);
+            const uint4 r = philox(make_uint4((uint32_t)quad, (uint32_t)(quad >> 32), (uint32_t)t,
+                                              (uint32_t)((uint64_t)t >> 32)), a.keys);
             const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
-            uint32_t mc = 0, vc = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              mc |= encode<true>(m[q][i], mi, rr[i] & 0xffffu) << (8 * i);
-              vc |= encode<false>(v[q][i], vi, rr[i] >> 16) << (8 * i);
-            }
+            const uint32_t mc = encode<true>(m[q], mi, rr, mtop), vc = encode<false>(v[q], vi, rr, vtop);
             *reinterpret_cast<uint32_t*>((uint8_t*)a.m + s0 + q * 128) = mc;
             *reinterpret_cast<uint32_t*>((uint8_t*)a.v + s0 + q * 128) = vc;
           }
@@ -347,31 +398,42 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(const __grid_constant__
   if (s_last) {
     if (!skip)
       for (int i = threadIdx.x; i < a.tensors; i += kThreads)
-        if (list.t[i].grad != nullptr) a.steps[a.tensor0 + i] += 1;
+        if (list.t[i].grad != nullptr) {
+          const int64_t t = a.steps[a.tensor0 + i] + 1;
+          a.steps[a.tensor0 + i] = t;
+          a.rates[a.tensor0 + i] = rate_of(t + 1, a.log_b1, a.log_b2, a.b1, a.b2);
+        }
     if (threadIdx.x == 0) a.ws->step_ticket = 0;
   }
 }
 
-// Values of 8-bit moments as BF16: four significant bits times a power of two.
-__global__ void __launch_bounds__(kThreads) decode_kernel(const uint8_t* __restrict__ m, const uint8_t* __restrict__ v,
+// Values of 8-bit moments as BF16: four significant bits times a power of two.  16 values per thread.
+__global__ void __launch_bounds__(kThreads) decode_kernel(const uint4* __restrict__ m, const uint4* __restrict__ v,
                                                           const uint8_t* __restrict__ m_scale,
                                                           const uint8_t* __restrict__ v_scale,
-                                                          uint32_t* __restrict__ m_out, uint32_t* __restrict__ v_out,
-                                                          int64_t quads) {
-  const int64_t q = (int64_t)blockIdx.x * kThreads + threadIdx.x;
-  if (q >= quads) return;
-  const int64_t block = q / (kBlockValues / 4);
+                                                          uint4* __restrict__ m_out, uint4* __restrict__ v_out,
+                                                          int64_t groups) {
+  const int64_t k = (int64_t)blockIdx.x * kThreads + threadIdx.x;
+  if (k >= groups) return;
+  const int64_t block = k / (kBlockValues / 16);
+  const uint4 mc = __ldcs(m + k), vc = __ldcs(v + k);
   const float ms = __uint_as_float((uint32_t)m_scale[block] << 23);
   const float vs = __uint_as_float((uint32_t)v_scale[block] << 23);
-  const uint32_t mc = reinterpret_cast<const uint32_t*>(m)[q], vc = reinterpret_cast<const uint32_t*>(v)[q];
-  uint32_t mo[4], vo[4];
+  const uint32_t mw[4] = {mc.x, mc.y, mc.z, mc.w}, vw[4] = {vc.x, vc.y, vc.z, vc.w};
+  uint32_t mo[8], vo[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    mo[i] = __float_as_uint(decode<true>((mc >> (8 * i)) & 255u, ms)) >> 16;
-    vo[i] = __float_as_uint(decode<false>((vc >> (8 * i)) & 255u, vs)) >> 16;
+  for (int i = 0; i < 8; ++i) {
+    const int j = 2 * (i & 1);
+    // the upper halves of two FP32 values side by side
+    mo[i] = __byte_perm(__float_as_uint(decode<true>(mw[i / 2], j, ms)),
+                        __float_as_uint(decode<true>(mw[i / 2], j + 1, ms)), 0x7632);
+    vo[i] = __byte_perm(__float_as_uint(decode<false>(vw[i / 2], j, vs)),
+                        __float_as_uint(decode<false>(vw[i / 2], j + 1, vs)), 0x7632);
   }
-  reinterpret_cast<uint2*>(m_out)[q] = make_uint2(mo[0] | mo[1] << 16, mo[2] | mo[3] << 16);
-  reinterpret_cast<uint2*>(v_out)[q] = make_uint2(vo[0] | vo[1] << 16, vo[2] | vo[3] << 16);
+  m_out[2 * k] = make_uint4(mo[0], mo[1], mo[2], mo[3]);
+  m_out[2 * k + 1] = make_uint4(mo[4], mo[5], mo[6], mo[7]);
+  v_out[2 * k] = make_uint4(vo[0], vo[1], vo[2], vo[3]);
+  v_out[2 * k + 1] = make_uint4(vo[4], vo[5], vo[6], vo[7]);
 }
 
 int launched(const char* what) {
@@ -435,12 +497,12 @@ extern "C" int ictc_adamw_grad_norm(const void* const* grads, int tensors, const
 
 extern "C" int ictc_adamw_step(void* const* weights, const void* const* grads, int first_tensor, int tensors,
                                const int32_t* chunks, const int64_t* first_chunk, int bits, void* m, void* v,
-                               uint8_t* m_scale, uint8_t* v_scale, float* average, int64_t* steps, double lr,
+                               uint8_t* m_scale, uint8_t* v_scale, float* average, int64_t* steps, void* rates, double lr,
                                double beta1, double beta2, double eps, double weight_decay, double average_decay,
                                uint64_t seed, int use_norm, void* workspace, void* stream) {
   if (bad_list(weights, grads, first_tensor, tensors, chunks, first_chunk, workspace, true) ||
       (bits != 8 && bits != 32) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) ||
-      !((float)eps > 0.f) || (tensors > 0 && (!steps || !m || !v || (bits == 8 && (!m_scale || !v_scale)))))
+      !((float)eps > 0.f) || (tensors > 0 && (!steps || !rates || !m || !v || (bits == 8 && (!m_scale || !v_scale)))))
     return invalid("ictc_adamw_step: invalid argument%s");
   Args a{};
   a.chunks = reinterpret_cast<const int4*>(chunks);
@@ -450,6 +512,7 @@ extern "C" int ictc_adamw_step(void* const* weights, const void* const* grads, i
   a.v_scale = v_scale;
   a.average = average;
   a.steps = steps;
+  a.rates = static_cast<Rate*>(rates);
   a.ws = static_cast<Workspace*>(workspace);
   a.use_norm = use_norm;
   a.b1 = (float)beta1;
@@ -460,11 +523,11 @@ extern "C" int ictc_adamw_step(void* const* weights, const void* const* grads, i
   a.keep = (float)(1.0 - lr * weight_decay);
   a.avg = (float)average_decay;
   a.avg1 = (float)(1.0 - average_decay);
-  a.lr = lr;
+  a.lr = (float)lr;
   a.log_b1 = log(beta1);
   a.log_b2 = log(beta2);
-  a.seed_lo = (uint32_t)seed;
-  a.seed_hi = (uint32_t)(seed >> 32);
+  for (uint32_t r = 0; r < kRounds; ++r)
+    a.keys[r] = make_uint2((uint32_t)seed + r * 0x9E3779B9u, (uint32_t)(seed >> 32) + r * 0xBB67AE85u);
   const int end = first_tensor + tensors;
   for (int t0 = first_tensor; t0 < end; t0 += kList) {
     TensorList list{};
@@ -496,9 +559,9 @@ extern "C" int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_
   if (values < 0 || values % kBlockValues || (values > 0 && (!m || !v || !m_scale || !v_scale || !m_out || !v_out)))
     return invalid("ictc_adamw_decode: invalid argument%s");
   if (values == 0) return ICTC_OK;
-  const int64_t quads = values / 4, grid = (quads + kThreads - 1) / kThreads;
+  const int64_t groups = values / 16, grid = (groups + kThreads - 1) / kThreads;
   if (grid > 0x7fffffff) return invalid("ictc_adamw_decode: too many values%s");
   decode_kernel<<<(unsigned)grid, kThreads, 0, (cudaStream_t)stream>>>(
-      (const uint8_t*)m, (const uint8_t*)v, m_scale, v_scale, (uint32_t*)m_out, (uint32_t*)v_out, quads);
+      (const uint4*)m, (const uint4*)v, m_scale, v_scale, (uint4*)m_out, (uint4*)v_out, groups);
   return launched("ictc_adamw_decode: %s");
 }

@@ -63,7 +63,7 @@ _SIGNATURES = {
     "ictc_adamw_chunk_values": [],
     "ictc_adamw_workspace_bytes": [],
     "ictc_adamw_grad_norm": [_p, _i, _p, _p, _f, _i, _i, _p, _p],
-    "ictc_adamw_step": [_p, _p, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _d, _u64, _i, _p,
+    "ictc_adamw_step": [_p, _p, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _d, _u64, _i, _p,
                         _p],
     "ictc_block_partial_floats": [_i, _i],
     "ictc_block_supported": [_i, _i],

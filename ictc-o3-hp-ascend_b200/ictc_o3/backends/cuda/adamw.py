@@ -57,7 +57,7 @@ class TensorTable:
     def step(self, weights, grads, first, count, bits, state, *, lr, betas, eps, weight_decay, ema_decay, seed,
              use_norm):
         launch(self.chunks.device, "ictc_adamw_step", weights, grads, first, count, self.chunks, self.first_chunk, bits,
-               state["m"], state["v"], state["m_scale"], state["v_scale"], state["average"], state["steps"], lr,
+               state["m"], state["v"], state["m_scale"], state["v_scale"], state["average"], state["steps"], state["rates"], lr,
                betas[0], betas[1], eps, weight_decay, ema_decay, seed, use_norm, self.workspace)
 
     def decode(self, state):

@@ -100,7 +100,8 @@ class AdamW(torch.optim.Optimizer):
             kind = torch.float32 if self.state_bits == 32 else torch.uint8
             flat = {"m": torch.zeros(table.values, dtype=kind, device=device),
                     "v": torch.zeros(table.values, dtype=kind, device=device), "m_scale": None, "v_scale": None,
-                    "average": None, "steps": torch.zeros(len(params), dtype=torch.int64, device=device)}
+                    "average": None, "steps": torch.zeros(len(params), dtype=torch.int64, device=device),
+                    "rates": torch.zeros(len(params), 4, dtype=torch.int64, device=device)}
             if self.state_bits == 8:
                 flat["m_scale"] = torch.ones(table.blocks, dtype=torch.uint8, device=device)
                 flat["v_scale"] = torch.ones(table.blocks, dtype=torch.uint8, device=device)
@@ -154,7 +155,6 @@ class AdamW(torch.optim.Optimizer):
         return (array("Q", [p.data_ptr() for p in params]),
                 array("Q", [0 if g is None else g.data_ptr() or self._empty for g in grads]), live, kept)
 
-    @torch.no_grad()
     def step(self, closure=None):
         loss = None
         if closure is not None:

@@ -363,7 +363,9 @@ int ictc_neighbor_list_noalloc(const float* pos, int64_t atoms, const float* box
  * State arrays hold the tensors one after another, each starting at a multiple of 256
  * values and padded with zeros to one:
  *   bits = 32  m, v FP32;  bits = 8  m, v one byte per value, m_scale, v_scale one
- *   byte per 256 values;  average FP32 or NULL;  steps device int64 [tensors]
+ *   byte per 256 values;  average FP32 or NULL;  steps device int64 [tensors];  rates
+ *   device [tensors][32 bytes], 32-byte aligned, zeroed once (bias corrections for the next
+ *   step, kept by the kernel)
  * `weights` and `grads` are host arrays of device pointers, read before the call
  * returns; a NULL gradient leaves its tensor (and its step count) alone.
  * `workspace`: ictc_adamw_workspace_bytes() device bytes, zeroed once, one per
@@ -383,8 +385,8 @@ int ictc_adamw_grad_norm(const void* const* grads, int tensors, const int32_t* c
                          float max_norm, int clip, int skip_nonfinite, void* workspace, void* stream);
 int ictc_adamw_step(void* const* weights, const void* const* grads, int first_tensor, int tensors,
                     const int32_t* chunks, const int64_t* first_chunk, int bits, void* m, void* v, uint8_t* m_scale,
-                    uint8_t* v_scale, float* average, int64_t* steps, double lr, double beta1, double beta2,
-                    double eps, double weight_decay, double average_decay, uint64_t seed, int use_norm,
+                    uint8_t* v_scale, float* average, int64_t* steps, void* rates, double lr, double beta1,
+                    double beta2, double eps, double weight_decay, double average_decay, uint64_t seed, int use_norm,
                     void* workspace, void* stream);
 
 /* Values (BF16, exact) that 8-bit moments stand for; values is a multiple of 256. */

@@ -21,7 +21,8 @@ def step(w, g, m, v, t, *, lr, betas, eps, weight_decay, clip=1.0):
     return w * (1 - lr * weight_decay) - update, m, v
 
 
-def step_bounds(w, g, m, v, t, *, lr, betas, eps, weight_decay, clip=1.0, clipped=False):
+def step_bounds(w, g, m, v, t, *, lr, betas, eps, weight_decay, clip=1.0, clipped=False,
+                approximate=False):
     """Largest rounding errors of an FP32 evaluation of ``step`` (elementwise, first order).
 
     Units of U.  g' = clip g: 1 for the product; clip itself 4 (norm, + 1e-6, reciprocal,
@@ -29,6 +30,9 @@ def step_bounds(w, g, m, v, t, *, lr, betas, eps, weight_decay, clip=1.0, clippe
     the sum 1: 3 |b1 m| + (3 + e) |(1-b1) g'|, e = error of g'.  v: g'^2 has 1 + 2e, then as
     m.  sqrt halves v's error; + 1 for itself, 1 for the constant 1/sqrt(1-b2^t), 1 for the
     product, 1 for + eps, 1 for eps itself.  The quotient 1, lr/(1-b1^t) 1, the product 1.
+    ``approximate``: root and quotient by hardware approximations, each within 2 units in the last
+    place = 4 half steps instead of 1 (root's and denominator's flush of values below 2^-126 included
+    in eps: eps >= 2^-126 / U is assumed).
     Weights: constant 1, product 1, difference 1."""
     b1, b2 = betas
     e = 5.0 if clipped else 0.0
@@ -38,9 +42,10 @@ def step_bounds(w, g, m, v, t, *, lr, betas, eps, weight_decay, clip=1.0, clippe
     dv = U * (3 * b2 * v + (4 + 2 * e) * (1 - b2) * gp * gp)
     size, root = lr / (1 - b1 ** t), v1.sqrt() / math.sqrt(1 - b2 ** t)
     den = root + eps
-    dden = 0.5 * dv / v1.clamp_min(1e-300) * root + U * 5 * den
+    more = 3 if approximate else 0
+    dden = 0.5 * dv / v1.clamp_min(1e-300) * root + U * (5 + more) * den
     update = size * m1.abs() / den
-    dupdate = size * dm / den + update * (dden / den + 3 * U)
+    dupdate = size * dm / den + update * (dden / den + (3 + more) * U)
     dw = dupdate + U * 3 * (w.abs() + update)
     return 1.01 * dw, 1.01 * dm, 1.01 * dv
 

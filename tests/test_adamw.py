@@ -70,16 +70,16 @@ def test_native_entry_points_validate_before_launching():
     first = (ctypes.c_int64 * 2)(0, 1)
     ones = (ctypes.c_void_p * 1)(1)
     some = ctypes.c_void_p(1)
-    common = [first, 32, some, some, None, None, None, some, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 0]
+    common = [first, 32, some, some, None, None, None, some, some, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 0]
 
     def step(**change):
-        names = ["first_chunk", "bits", "m", "v", "m_scale", "v_scale", "average", "steps", "lr", "b1", "b2", "eps",
+        names = ["first_chunk", "bits", "m", "v", "m_scale", "v_scale", "average", "steps", "rates", "lr", "b1", "b2", "eps",
                  "wd", "avg", "seed", "use_norm"]
         values = dict(zip(names, common), **change)
         return lib.ictc_adamw_step(change.pop("weights", ones), ones, 0, 1, some, *[values[n] for n in names], some,
                                    None)
 
-    for change in ({"bits": 16}, {"bits": 8}, {"m": None}, {"steps": None}, {"b1": 1.0}, {"b2": -0.1}, {"eps": 0.0},
+    for change in ({"bits": 16}, {"bits": 8}, {"m": None}, {"steps": None}, {"rates": None}, {"b1": 1.0}, {"b2": -0.1}, {"eps": 0.0},
                    {"eps": 1e-50}, {"first_chunk": None}):
         assert step(**change) == -1, change
         assert "invalid" in lib.ictc_last_error().decode()
