@@ -38,8 +38,8 @@ void ictc_set_error(const char* fmt, const char* detail);
 namespace ictc {
 namespace {
 
-constexpr int kThreads = 256;
-constexpr int kChunk = 2048;          // values per block: 8 per thread
+constexpr int kThreads = 128;
+constexpr int kChunk = 1024;          // values per block: 8 per thread
 constexpr int kQuads = 2;             // groups of 4 values per thread
 constexpr int kBlockValues = 256;     // values that share a scale: 32 lanes x 8
 constexpr int kNormBlocks = 1184;     // partial sums of the gradient norm at most
@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
 }
 
 template <int BITS, bool AVERAGE>
-__global__ void __launch_bounds__(kThreads, 4) adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
+__global__ void __launch_bounds__(kThreads, BITS == 8 ? 9 : 8) adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
   __shared__ int s_last;
   const int4 c = a.chunks_n ? a.chunks[a.chunk0 + blockIdx.x] : make_int4(a.tensor0, 0, 0, 0);
   const Tensor tensor = list.t[c.x - a.tensor0];
