@@ -100,6 +100,7 @@ class DegreeNorm(torch.nn.Module):
     def __init__(self, channels, lmax, *, layout="mul_ir", eps=1e-6):
         super().__init__()
         self.channels, self.lmax, self.layout, self.eps = channels, lmax, layout, eps
+        self.form = _form(channels, lmax, layout, eps, True)
         self.weight = torch.nn.Parameter(torch.ones(lmax + 1, channels))
 
     def forward(self, features):
@@ -115,6 +116,7 @@ class ResidualBlockNorm(torch.nn.Module):
     def __init__(self, channels, lmax, *, next_norm=True, scale_init=1.0, layout="mul_ir", eps=1e-6):
         super().__init__()
         self.channels, self.lmax, self.layout, self.eps = channels, lmax, layout, eps
+        self.form = _form(channels, lmax, layout, eps, bool(next_norm))
         self.post_weight = torch.nn.Parameter(torch.ones(lmax + 1, channels))
         self.scale = torch.nn.Parameter(torch.full((lmax + 1, channels), float(scale_init)))
         self.pre_weight = torch.nn.Parameter(torch.ones(lmax + 1, channels)) if next_norm else None

@@ -135,6 +135,7 @@ def from_reference_state_dict(model, state: Dict[str, torch.Tensor], strict: boo
     as identities or as constants this model does not need.  With ``strict``,
     unknown keys and missing parameters raise."""
     from ictc_o3.ops.symmetric_contraction import ICTDBridgeUSymmetricContractionSO3
+    _check_no_block_norm(model)
     own = dict(model.named_parameters())
     own.update(dict(model.named_buffers()))
     target: Dict[str, torch.Tensor] = {}
@@ -241,6 +242,11 @@ def from_reference_state_dict(model, state: Dict[str, torch.Tensor], strict: boo
     return accepted
 
 
+def _check_no_block_norm(model):
+    if getattr(model, "block_norm", False):
+        raise ValueError("a model with block norms has no counterpart in the reference")
+
+
 # Architecture metadata a reference checkpoint must carry (the keys the reference's
 # multi-device engine requires, ``mace_ictc/interfaces/ascend_lammps.py:50-53``).
 # Product backends whose checkpoints load onto this model (either backend): by name,
@@ -268,6 +274,7 @@ def check_reference_metadata(model, metadata: Dict[str, object]):
     radial embedding's sqrt(num_basis) factor has no parameter), so a checkpoint
     whose metadata is missing or differs is refused rather than loaded into a model
     that would give different energies."""
+    _check_no_block_norm(model)
     missing = [k for k in REQUIRED_METADATA if k not in metadata]
     if missing:
         raise ValueError(f"Missing model metadata: {missing}; re-save with the training configuration")
@@ -305,6 +312,7 @@ def load_reference_checkpoint(model, checkpoint: Dict[str, object], strict: bool
 
 def to_reference_state_dict(model) -> Dict[str, torch.Tensor]:
     """The inverse mapping: a state dict with the reference's names and layouts."""
+    _check_no_block_norm(model)
     out: Dict[str, torch.Tensor] = {"node_embedding.weight": model.node_embedding.weight.detach().clone()}
     for i, block in enumerate(model.interactions):
         p = f"interactions.{i}"

@@ -15,7 +15,10 @@ Structure of the reference model (``mace_ictc/models/pure_cartesian_ictd_fix.py`
   targets are lmax for every layer but the last, which targets scalars;
 * energy readouts: a linear scalar readout per intermediate layer, an MLP
   readout (C -> 16 -> 1, normalised SiLU) after the last (:1400-1420, :3070-3100);
-* forces = -dE/dpos (``mace_ictc/hp/runtime.py:84-121``).
+* forces = -dE/dpos (``mace_ictc/hp/runtime.py:84-121``);
+* with ``block_norm`` (no counterpart in the reference's two-layer models) every block reads
+  normed rows, and its product is normed, gated and scaled before it joins the
+  self-connection: h' = sc + scale * sigmoid(gate) * post * norm(product), next input pre * norm(h').
 
 The three hot operators (edge harmonics, TP graph message, symmetric
 contraction) are taken from an ``ops`` object; the default is the CUDA backend.
@@ -57,6 +60,13 @@ class CudaOps:
 
     def contraction(self, module, features, species):
         return module(features, node_type_idx=species)
+
+    def block_end(self, norm, stream, branch, gate):
+        """(stream behind a block, next block's normed rows or None): one fused kernel each way."""
+        return norm(stream, branch, gate)
+
+    def block_start(self, norm, features):
+        return norm(features)
 
     def radial(self, fc, feats):
         """Gates of the radial MLP on the fused tensor-core kernels; a shape the kernels do
@@ -224,9 +234,10 @@ class InteractionBlock(nn.Module):
                                                                                   init="identity")
 
     def forward(self, ops, node_feats, edge_harmonics, edge_feats, src, dst, mask, groups, owned=None,
-                species=None, exchange=None):
+                species=None, exchange=None, stream=None):
         """Messages into the first ``owned`` nodes (all nodes by default); ``groups`` and
         ``species`` (the owned nodes' species) select the element-conditioned weights.
+        ``stream``: rows for the self-connection where they are not ``node_feats`` (block norms).
 
         With ``exchange`` (spatial decomposition), ``node_feats`` holds the owned rows
         only: ``linear_up`` runs on them (it acts row by row, so it commutes with the
@@ -243,7 +254,7 @@ class InteractionBlock(nn.Module):
         message = self.message_linear(msg, scale=1.0 / max(self.avg_num_neighbors, 1e-8))
         if self.self_connection is None:
             return self.message_selector(message, groups, species), None
-        sc_in = node_feats[:owned, :self.channels * (self.sc_lmax + 1) ** 2]
+        sc_in = (node_feats if stream is None else stream)[:owned, :self.channels * (self.sc_lmax + 1) ** 2]
         return message, self.self_connection(sc_in, groups, species)
 
 
@@ -260,8 +271,12 @@ class ProductBlock(nn.Module):
             correlation=correlation)
         self.linear = ChannelLinearSO3(channels, channels, target_lmax)
 
+    def branch(self, ops, message, species):
+        """The block's own rows, without the self-connection."""
+        return self.linear(ops.contraction(self.symmetric_contractions, message, species))
+
     def forward(self, ops, message, sc, species):
-        out = self.linear(ops.contraction(self.symmetric_contractions, message, species))
+        out = self.branch(ops, message, species)
         if sc is not None:
             if sc.shape[-1] == out.shape[-1]:
                 out = out + sc
@@ -276,7 +291,7 @@ class MACEICTC(nn.Module):
     def __init__(self, *, num_elements=None, channels=64, lmax=2, num_interactions=2, correlation=3, r_max=5.0,
                  num_basis=8, polynomial_cutoff_p=5, avg_num_neighbors=1.0, readout_hidden=16, ops=None,
                  atomic_numbers=(1, 6, 8), first_layer_self_connection=True, radial_sqrt_num_basis=False,
-                 product_backend="ictd-pure-u"):
+                 product_backend="ictd-pure-u", block_norm=False, block_scale=1.0):
         """Defaults follow the reference constructor for new models: atomic numbers
         H, C, O (``mace_ictc/hp/runtime.py:7``), an element-conditioned scalar
         self-connection in the first layer (``mace_ictc/models/factory.py:17``,
@@ -290,11 +305,19 @@ class MACEICTC(nn.Module):
         :2166): "ictd-pure-u" (ICTC couplings) or "ictd-bridge-u" (the reference's
         default; the couplings are buffers that its checkpoints overwrite).  Both run
         the same kernels and span the same couplings; checkpoints of either load
-        into a model of either."""
+        into a model of either.
+
+        ``block_norm`` adds norms before and after every block with a gate and a residual
+        scale that starts at ``block_scale`` (``ictc_o3.ops.block_norm``), for stacks whose
+        activations would grow from layer to layer.  Such a model is this package's own:
+        reference checkpoints neither load into it nor are written from it."""
         super().__init__()
         if product_backend not in PRODUCT_MODULES:
             raise ValueError(f"product_backend must be one of {tuple(PRODUCT_MODULES)}")
+        if block_norm and not first_layer_self_connection:
+            raise ValueError("block_norm requires first_layer_self_connection")
         self.product_backend = product_backend
+        self.block_norm = bool(block_norm)
         atomic_numbers = tuple(sorted({int(z) for z in atomic_numbers}))
         if not atomic_numbers or atomic_numbers[0] < 0:
             raise ValueError("atomic_numbers must be non-negative and not empty")
@@ -330,6 +353,15 @@ class MACEICTC(nn.Module):
                                              for _ in range(num_interactions - 1)])
         self.last_readout = nn.Sequential(nn.Linear(channels, readout_hidden, bias=False), NormalizedSiLU(),
                                           nn.Linear(readout_hidden, 1, bias=False))
+        if self.block_norm:
+            from ictc_o3.ops.block_norm import DegreeNorm, ResidualBlockNorm
+            targets = [p.target_lmax for p in self.products]
+            self.input_norm = DegreeNorm(channels, 0)
+            self.block_norms = nn.ModuleList([ResidualBlockNorm(channels, t, next_norm=i + 1 < num_interactions,
+                                                                scale_init=block_scale)
+                                              for i, t in enumerate(targets)])
+            # gates of a block's degrees and channels from its message's scalars
+            self.block_gates = nn.ModuleList([ChannelLinearSO3(channels, (t + 1) * channels, 0) for t in targets])
 
     @staticmethod
     def edge_vectors(pos, src, dst, shift_vectors=None):
@@ -351,6 +383,27 @@ class MACEICTC(nn.Module):
 
     def edge_inputs(self, pos, src, dst, shift_vectors):
         return self.edge_features(self.edge_vectors(pos, src, dst, shift_vectors))
+
+    def _block_start(self, features):
+        run = getattr(self.ops, "block_start", None)
+        if run is not None:
+            return run(self.input_norm, features)
+        from ictc_o3.backends.cuda.block_norm import formula
+        norm = self.input_norm
+        return formula(norm.form, features, None, None, None, None, norm.weight)[1]
+
+    def _block_end(self, layer, message, sc, species):
+        """(stream, normed rows of the next block) behind block ``layer``."""
+        branch = self.products[layer].branch(self.ops, message, species)
+        if sc.shape[1] != branch.shape[1]:      # the first self-connection has scalars only
+            sc = F.pad(sc, (0, branch.shape[1] - sc.shape[1]))
+        gate = self.block_gates[layer](message[:, :self.channels])
+        norm = self.block_norms[layer]
+        run = getattr(self.ops, "block_end", None)
+        if run is not None:
+            return run(norm, sc, branch, gate)
+        from ictc_o3.backends.cuda.block_norm import formula
+        return formula(norm.form, sc, branch, gate, norm.post_weight, norm.scale, norm.pre_weight)
 
     def node_energies(self, pos, species, src, dst, shift_vectors=None, layers=None):
         """Per-node energies [N] (sum of the layer readouts)."""
@@ -388,11 +441,16 @@ class MACEICTC(nn.Module):
         h = self.node_embedding.weight.t().index_select(0, species)
         energy = None
         count = len(self.interactions) if layers is None else layers
+        normed = self._block_start(h) if self.block_norm else None
         for layer in range(count):
-            message, sc = self.interactions[layer](self.ops, h, harmonics, feats, src, dst, mask, groups, owned,
-                                                   own_species, exchange=exchange if layer else None)
+            message, sc = self.interactions[layer](self.ops, h if normed is None else normed, harmonics, feats, src,
+                                                   dst, mask, groups, owned, own_species,
+                                                   exchange=exchange if layer else None, stream=h)
             mark(f"layer{layer}.interaction")
-            h = self.products[layer](self.ops, message, sc, own_species)
+            if self.block_norm:
+                h, normed = self._block_end(layer, message, sc, own_species)
+            else:
+                h = self.products[layer](self.ops, message, sc, own_species)
             readout = (self.layer_readouts[layer](h[:, :self.channels]) if layer < len(self.interactions) - 1
                        else self.last_readout(h[:, :self.channels]))
             energy = readout if energy is None else energy + readout
