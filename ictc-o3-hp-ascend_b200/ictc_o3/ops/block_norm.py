@@ -45,10 +45,15 @@ def _form(channels, lmax, layout, eps, norm):
 def _check(form, rows, weights, gate=None):
     c, degrees = form.channels, form.lmax + 1
     n = rows[0].shape[0] if rows[0].ndim else 0
-    require_cuda_fp32(*rows, *weights, *(() if gate is None else (gate,)))
-    if any(x.shape != (n, c * degrees * degrees) for x in rows):
+    tensors = [*rows, *weights] if gate is None else [*rows, *weights, gate]
+    index = rows[0].get_device()
+    if index < 0 or any([t.dtype is not torch.float32 or t.get_device() != index for t in tensors]):
+        require_cuda_fp32(*tensors)
+    require_cuda_fp32(rows[0])      # and the modes that forbid it
+    width, shape = (n, c * degrees * degrees), (degrees, c)
+    if any([x.shape != width for x in rows]):
         raise ValueError("Rows must have shape [N,C*(L+1)^2]")
-    if any(w.shape != (degrees, c) for w in weights):
+    if any([w.shape != shape for w in weights]):
         raise ValueError("Weights must have shape [L+1,C]")
     if gate is not None and gate.shape != (n, degrees * c) and gate.shape != (n, degrees, c):
         raise ValueError("Gates must have shape [N,(L+1)*C] or [N,L+1,C]")

@@ -133,27 +133,28 @@ class AdamW(torch.optim.Optimizer):
     def _gather(self):
         """Addresses of weights and gradients (0: no gradient), the updated weights, and
         temporaries that must outlive the launch."""
-        params = self._params
+        params, expected = self._params, self._expected
         grads = [p.grad for p in params]
-        live, expected, given, kept = params, self._expected, grads, ()
-        if any([g is None for g in grads]):
+        live, kept = params, ()
+        try:      # as a rule: a dense, contiguous gradient everywhere, found by one comparison
+            fine = [(g.dtype, g.get_device(), g.numel(), g.is_contiguous()) for g in grads] == expected
+            places = [g.data_ptr() for g in grads] if fine else None
+        except (AttributeError, RuntimeError):      # None, or a layout without an address
+            fine = False
+        if not fine:
             live = [p for p, g in zip(params, grads) if g is not None]
-            expected = [e for e, g in zip(self._expected, grads) if g is not None]
-            given = [g for g in grads if g is not None]
-        # one comparison of all at once; what differs is looked at below
+            expected = [e for e, g in zip(expected, grads) if g is not None]
         if [(p.dtype, p.get_device(), p.numel(), p.is_contiguous()) for p in live] != expected:
             raise ValueError("a parameter has changed its type, device, size or layout since the optimizer was built")
-        if any([g.is_sparse for g in given]) or (
-                [(g.dtype, g.get_device(), g.numel(), g.is_contiguous()) for g in given] != expected):
-            for g, e in zip(given, expected):
+        if not fine:
+            for g, e in zip([g for g in grads if g is not None], expected):
                 if g.layout is not torch.strided or (g.dtype, g.get_device(), g.numel()) != e[:3]:
                     raise ValueError("gradients must be dense CUDA FP32 tensors of their parameter's size")
-            grads = kept = [None if g is None else g.detach().contiguous() for g in grads]
-        if live is params and self._full:
-            return array("Q", [p.data_ptr() for p in params]), array("Q", [g.data_ptr() for g in grads]), live, kept
-        # a tensor without values has no address, but its steps count
-        return (array("Q", [p.data_ptr() for p in params]),
-                array("Q", [0 if g is None else g.data_ptr() or self._empty for g in grads]), live, kept)
+            kept = [None if g is None else g.detach().contiguous() for g in grads]
+            places = [0 if g is None else g.data_ptr() for g in kept]
+        if not self._full:      # a tensor without values has no address, but its steps count
+            places = [self._empty if g is not None and not g.numel() else k for g, k in zip(grads, places)]
+        return array("Q", [p.data_ptr() for p in params]), array("Q", places), live, kept
 
     def step(self, closure=None):
         loss = None

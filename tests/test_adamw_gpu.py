@@ -364,6 +364,10 @@ def test_refusals(cuda_device):
     with pytest.raises(TypeError):
         opt.step()
     opt.param_groups[0]["lr"] = 1e-3
+    q = torch.nn.Parameter(torch.zeros(64, device=cuda_device))
+    q.grad = torch.zeros(64, device=cuda_device).to_sparse()
+    with pytest.raises(ValueError, match="dense"):
+        AdamW([q]).step()
     p.grad = None
     p.data = torch.zeros(32, device=cuda_device)
     p.grad = torch.zeros(32, device=cuda_device)
