@@ -237,16 +237,29 @@ class AdamW(torch.optim.Optimizer):
                 if key == "step":
                     if int(theirs) < 0:
                         raise ValueError("a step count is negative")
-                elif theirs.dtype != value.dtype or theirs.shape != value.shape:
+                elif not isinstance(theirs, torch.Tensor) or theirs.dtype != value.dtype or theirs.shape != value.shape:
                     raise ValueError(f"{key} has another type or shape; was it saved with other state_bits?")
+                elif key.endswith("exponent") and theirs.numel() and (int(theirs.min()) < 1 or int(theirs.max()) > 253):
+                    raise ValueError(f"{key} is outside 1..253")
         for group, values in zip(self.param_groups, loaded):
             group.update(values, betas=tuple(values["betas"]))
+        steps, to, values = [], [], []
         for name, p in zip(names, self._params):
             entry, mine = saved.get(name), self.state[p]
+            steps.append(0 if entry is None else int(entry["step"]))
             for key, value in mine.items():
+                if key == "step":
+                    continue
                 if entry is not None and key in entry:
-                    value.fill_(int(entry[key])) if key == "step" else value.copy_(entry[key])
+                    to.append(value)
+                    values.append(entry[key])
                 elif key == "ema":
                     value.copy_(p)
                 else:
                     value.fill_(1 if key.endswith("exponent") else 0)
+        self._flat["steps"].copy_(torch.tensor(steps, dtype=torch.int64))
+        if all(v.device == self._device for v in values):
+            torch._foreach_copy_(to, values)
+        else:
+            for mine, value in zip(to, values):
+                mine.copy_(value)

@@ -332,6 +332,10 @@ def test_state_dicts(cuda_device):
                                                                                 other.state[q].values()))
     with pytest.raises(ValueError, match="state_bits"):
         AdamW(make([700, 3], cuda_device), state_bits=8).load_state_dict(AdamW(make([700, 3], cuda_device)).state_dict())
+    bad = copy.deepcopy(opt.state_dict())
+    bad["state"][0]["exp_avg_exponent"][0] = 255
+    with pytest.raises(ValueError, match="1..253"):
+        opt.load_state_dict(bad)
     with pytest.raises(ValueError, match="parameter groups"):
         AdamW(make([700], cuda_device)).load_state_dict(opt.state_dict())
     # the library's own state continues here

@@ -243,6 +243,41 @@ def test_absent_cotangents(wanted, cuda_device):
     compare(29, 24, 2, "mul_ir", wanted=wanted, device=cuda_device)
 
 
+@pytest.mark.parametrize("frozen", [("stream",), ("branch", "gate"), ("stream", "branch", "gate"),
+                                    ("post_weight", "scale", "pre_weight"), ("stream", "branch", "scale", "pre_weight"),
+                                    ("gate", "post_weight", "pre_weight"), ("branch", "post_weight", "scale")])
+def test_frozen_arguments(frozen, cuda_device):
+    """Whatever does not require a gradient, the others receive the same ones."""
+    from ictc_o3.ops.block_norm import residual_block_norm
+    t = inputs(41, 24, 2, seed=9)
+    names = ["stream", "branch", "gate", "post_weight", "scale", "pre_weight"]
+
+    def run(values):
+        out = residual_block_norm(values["stream"], values["branch"], channels=24, lmax=2,
+                                  **{k: values[k] for k in names[2:]})
+        live = [k for k in names if values[k].requires_grad]
+        first = torch.autograd.grad(out, [values[k] for k in live], [t["p"], t["q"]], create_graph=True)
+        rows = [g for g, k in zip(first, live) if k in names[:3]]
+        found = dict(zip(live, first))
+        if rows:
+            dots = [t["d_" + k] for k in live if k in names[:3]]
+            second = torch.autograd.grad(rows, [values[k] for k in live], dots, allow_unused=True)
+            found |= {"dd " + k: g for k, g in zip(live, second)}
+        return found
+
+    some = {k: t[k].detach().requires_grad_(k not in frozen) for k in names}
+    got, full = run(some), run({k: t[k] for k in names})
+    for k, g in got.items():
+        if not k.startswith("dd ") and g is not None:
+            assert torch.equal(g, full[k]), k
+    zero = dict(t, **{"d_" + k: torch.zeros_like(t["d_" + k]) for k in names[:3] if k in frozen})
+    t.update(zero)                       # frozen rows have no cotangent of their gradient
+    full = run({k: t[k].detach().requires_grad_() for k in names})
+    for k, g in got.items():
+        if k.startswith("dd ") and g is not None:
+            assert torch.allclose(g, full[k], rtol=1e-5, atol=1e-5 * float(full[k].abs().max())), k
+
+
 @pytest.mark.parametrize("offset", [1, 2])
 @pytest.mark.parametrize("channels, lmax", [(64, 2), (50, 1), (7, 3)])
 def test_unaligned_views(channels, lmax, offset, cuda_device):

@@ -80,3 +80,40 @@ def test_optimizer_requires_the_device():
     from mace_ictc.training import create_optimizer
     with pytest.raises(ValueError):
         create_optimizer(_model(block_norm=True))
+
+
+def _normed_model():
+    from mace_ictc.models import MACEICTC
+    from oracle.model_ops import OracleOps
+    torch.manual_seed(12)
+    return MACEICTC(channels=8, lmax=2, num_interactions=3, r_max=3.0, avg_num_neighbors=5.0, ops=OracleOps(),
+                    block_norm=True, block_scale=0.5).double()
+
+
+def _rank(rank, world, port, out_dir, case):
+    import os
+    import test_parallel_cpu
+    test_parallel_cpu._model = _normed_model
+    if rank < world:
+        test_parallel_cpu._worker(rank, world, port, out_dir, case)
+    else:       # the single process, beside the ranks and with as many threads (coupling tables depend on them)
+        torch.set_num_threads(1)
+        torch.save(test_parallel_cpu._single(*test_parallel_cpu._system(**case["system"])),
+                   os.path.join(out_dir, "single.pt"))
+
+
+def test_slab_decomposition_with_block_norms(tmp_path):
+    """Norms act row by row, so ranks with halos give the single process's energy and forces."""
+    import torch.multiprocessing as mp
+    from test_parallel_cpu import _free_port
+    case = {"system": {"n_atoms": 60, "seed": 4}}
+    mp.start_processes(_rank, args=(2, _free_port(), str(tmp_path), case), nprocs=3, join=True, start_method="spawn")
+    outs = [torch.load(tmp_path / f"rank{r}.pt") for r in range(2)]
+    energy, forces, virial = torch.load(tmp_path / "single.pt")
+    joined = torch.empty_like(forces)
+    for out in outs:
+        joined[out["ids"]] = out["forces"]
+        # FP64 sums in another order (1e-15 each, some 1e3 terms) through three norms (1e3 times)
+        torch.testing.assert_close(out["energy"], energy, rtol=1e-9, atol=1e-9)
+        torch.testing.assert_close(out["virial"], virial, rtol=1e-8, atol=1e-8)
+    torch.testing.assert_close(joined, forces, rtol=1e-8, atol=1e-8)
