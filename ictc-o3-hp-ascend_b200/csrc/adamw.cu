@@ -7,10 +7,12 @@
 // clip = min(1, max_norm / (|g| + 1e-6)) comes from a first pass over the gradients
 // (grad_norm_kernel) when clipping or skipping of non-finite steps is asked for.
 //
-// Work is cut into chunks of kChunk consecutive values of one tensor; a static device
-// table gives each chunk's tensor, place and count, and the addresses of weights and
-// gradients travel in the kernel's parameters (they may change from step to step).
-// One block per chunk, eight values per thread.
+// Work is cut into chunks of consecutive values of one tensor; a static device table gives
+// each chunk's tensor, place and count, and the addresses of weights and gradients travel
+// in the kernel's parameters (they may change from step to step).  One block per chunk,
+// which it works off in turns of 1,024 values, eight per thread; how many turns a chunk
+// has goes by the total (the caller's rule): one where there are few values, since
+// latency counts, 16 where there are many, since a block's own costs then spread.
 //
 // 8-bit moments: blocks of 256 values (one warp's share) have a power-of-two scale
 // 2^(byte - 127), byte = exponent field of the block's largest magnitude + 1, limited to
@@ -39,14 +41,14 @@ namespace ictc {
 namespace {
 
 constexpr int kThreads = 128;
-constexpr int kChunk = 1024;          // values per block: 8 per thread
+constexpr int kTurn = 1024;           // values that a block works on at once: 8 per thread
 constexpr int kQuads = 2;             // groups of 4 values per thread
 constexpr int kBlockValues = 256;     // values that share a scale: 32 lanes x 8
 constexpr int kNormBlocks = 1184;     // partial sums of the gradient norm at most
 constexpr int kRounds = 7;            // of Philox: the fewest its authors report as passing their tests
 constexpr int kList = 240;            // tensors per launch: 16 B each, below 4 KB of parameters
 
-static_assert(kChunk == kThreads * kQuads * 4 && kBlockValues == 32 * kQuads * 4, "a warp owns one scale block");
+static_assert(kTurn == kThreads * kQuads * 4 && kBlockValues == 32 * kQuads * 4, "a warp owns one scale block");
 
 // A tensor's bias corrections for its next step, left behind by the last one: a block then reads
 // them with its values instead of waiting for one thread's FP64 exponentials (8-bit states, 160 M
@@ -87,6 +89,8 @@ struct Args {
   const int4* chunks;   // {tensor, values, first scale block, chunk of the tensor}
   int tensor0;          // the list's first tensor
   int tensors;
+  int chunk;            // values per chunk: kTurn << shift
+  int shift;
   int64_t chunk0;
   int64_t chunks_n;
   void* m;
@@ -212,26 +216,24 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
                                                              int clip, int skip_bad) {
   __shared__ double shared[kThreads / 32];
   __shared__ int last;
-  constexpr int kAhead = 4;      // chunks whose values are in flight together
+  constexpr int kAhead = 4;      // turns whose values are in flight together
   double sum = 0.0;
-  for (int64_t i0 = blockIdx.x; i0 < a.chunks_n; i0 += kAhead * (int64_t)gridDim.x) {
-    int4 c[kAhead];
+  const int64_t total = a.chunks_n << a.shift;
+  for (int64_t i0 = blockIdx.x; i0 < total; i0 += kAhead * (int64_t)gridDim.x) {
     float4 x[kAhead][kQuads];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int64_t i = i0 + k * (int64_t)gridDim.x;
-      c[k] = i < a.chunks_n ? a.chunks[a.chunk0 + i] : make_int4(a.tensor0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int k = 0; k < kAhead; ++k) {
-      const float* g = list.t[c[k].x - a.tensor0].grad;
-      if (g == nullptr) c[k].y = 0;
-      g += (int64_t)c[k].w * kChunk;
+      const int turn = (int)(i & ((1 << a.shift) - 1)) * kTurn;
+      const int4 c = i < total ? a.chunks[a.chunk0 + (i >> a.shift)] : make_int4(a.tensor0, 0, 0, 0);
+      const float* g = list.t[c.x - a.tensor0].grad;
+      const int count = g == nullptr ? 0 : c.y - turn;
+      g += (int64_t)c.w * a.chunk + turn;
       const bool al = aligned16(g);
 #pragma unroll
       for (int q = 0; q < kQuads; ++q) {
         const int at = (q * kThreads + threadIdx.x) * 4;
-        x[k][q] = load4(g + at, c[k].y - at, al);
+        x[k][q] = load4(g + at, count - at, al);
       }
     }
 #pragma unroll
@@ -269,123 +271,180 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
   }
 }
 
+// What a lane reads of one turn.
 template <int BITS, bool AVERAGE>
-__global__ void __launch_bounds__(kThreads, BITS == 8 ? 9 : 8) adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
+struct Turn {
+  float4 w[kQuads], g[kQuads], m[BITS == 32 ? kQuads : 1], v[BITS == 32 ? kQuads : 1], e[AVERAGE ? kQuads : 1];
+  uint32_t mc[BITS == 8 ? kQuads : 1], vc[BITS == 8 ? kQuads : 1];
+};
+
+// s0: place in the state arrays; left: values of the tensor from this lane's first one on.
+template <int BITS, bool AVERAGE>
+__device__ __forceinline__ void read(Turn<BITS, AVERAGE>& x, const Args& a, const float* w, const float* g, int64_t s0,
+                                     int left, bool fast, bool wal, bool gal) {
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    if (fast) {
+      x.g[q] = *reinterpret_cast<const float4*>(g + q * 128);
+      x.w[q] = *reinterpret_cast<const float4*>(w + q * 128);
+    } else {
+      x.g[q] = load4(g + q * 128, left - q * 128, gal);
+      x.w[q] = load4(w + q * 128, left - q * 128, wal);
+    }
+    if constexpr (BITS == 32) {
+      x.m[q] = *reinterpret_cast<const float4*>((const float*)a.m + s0 + q * 128);
+      x.v[q] = *reinterpret_cast<const float4*>((const float*)a.v + s0 + q * 128);
+    } else {
+      x.mc[q] = *reinterpret_cast<const uint32_t*>((const uint8_t*)a.m + s0 + q * 128);
+      x.vc[q] = *reinterpret_cast<const uint32_t*>((const uint8_t*)a.v + s0 + q * 128);
+    }
+    if constexpr (AVERAGE) x.e[q] = *reinterpret_cast<const float4*>(a.average + s0 + q * 128);   // padded
+  }
+}
+
+// mb, vb: the block's scale bytes, in and out.
+template <int BITS, bool AVERAGE>
+__device__ __forceinline__ void update(const Turn<BITS, AVERAGE>& x, const Args& a, float* wp, int64_t s0, int left,
+                                       bool fast, bool wal, float clip, float size, float rate, int64_t t,
+                                       uint32_t& mb, uint32_t& vb) {
+  float w[kQuads][4], m[kQuads][4], v[kQuads][4];
+  uint32_t mmax = 0, vmax = 0;      // as patterns: infinities and NaN are the largest
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    const float g[4] = {x.g[q].x, x.g[q].y, x.g[q].z, x.g[q].w}, ow[4] = {x.w[q].x, x.w[q].y, x.w[q].z, x.w[q].w};
+    float om[4], ov[4];
+    if constexpr (BITS == 32) {
+      om[0] = x.m[q].x; om[1] = x.m[q].y; om[2] = x.m[q].z; om[3] = x.m[q].w;
+      ov[0] = x.v[q].x; ov[1] = x.v[q].y; ov[2] = x.v[q].z; ov[3] = x.v[q].w;
+    } else {
+      const float ms = __uint_as_float(mb << 23), vs = __uint_as_float(vb << 23);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        om[i] = decode<true>(x.mc[q], i, ms);
+        ov[i] = decode<false>(x.vc[q], i, vs);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float y = __fmul_rn(g[i], clip);
+      m[q][i] = __fadd_rn(__fmul_rn(om[i], a.b1), __fmul_rn(y, a.c1));
+      v[q][i] = __fadd_rn(__fmul_rn(ov[i], a.b2), __fmul_rn(__fmul_rn(y, y), a.c2));
+      if constexpr (BITS == 8) {
+        mmax = max(mmax, __float_as_uint(fabsf(m[q][i])));
+        vmax = max(vmax, __float_as_uint(v[q][i]));      // a NaN of a sum of squares is positive
+        // bound by its instructions: hardware root and quotient (within 2 units in the last place)
+        float root;
+        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v[q][i]));
+        const float den = fmaf(root, rate, a.eps);
+        w[q][i] = fmaf(ow[i], a.keep, -size * __fdividef(m[q][i], den));
+      } else {
+        const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v[q][i]), rate), a.eps);
+        w[q][i] = __fsub_rn(__fmul_rn(ow[i], a.keep), __fmul_rn(size, __fdiv_rn(m[q][i], den)));
+      }
+    }
+  }
+  bool mtop = false, vtop = false;
+  float mi = 0.f, vi = 0.f;
+  if constexpr (BITS == 8) {
+    mmax = __reduce_max_sync(0xffffffffu, mmax);
+    vmax = __reduce_max_sync(0xffffffffu, vmax);
+    if (max(mmax, vmax) >= 0x7f800000u) return;      // the codes hold no NaN: the block stays as it was
+    mb = scale_byte(mmax);
+    vb = scale_byte(vmax);
+    mtop = mb == 253u;
+    vtop = vb == 253u;
+    mi = __uint_as_float((254u - mb) << 23);
+    vi = __uint_as_float((254u - vb) << 23);
+  }
+#pragma unroll
+  for (int q = 0; q < kQuads; ++q) {
+    if (fast) *reinterpret_cast<float4*>(wp + q * 128) = make_float4(w[q][0], w[q][1], w[q][2], w[q][3]);
+    else store4(wp + q * 128, w[q], left - q * 128, wal);
+    if constexpr (BITS == 32) {
+      *reinterpret_cast<float4*>((float*)a.m + s0 + q * 128) = make_float4(m[q][0], m[q][1], m[q][2], m[q][3]);
+      *reinterpret_cast<float4*>((float*)a.v + s0 + q * 128) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
+    } else {
+      const uint64_t quad = (uint64_t)(s0 + q * 128) >> 2;
+      const uint4 r = philox(make_uint4((uint32_t)quad, (uint32_t)(quad >> 32), (uint32_t)t,
+                                        (uint32_t)((uint64_t)t >> 32)), a.keys);
+      const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
+      *reinterpret_cast<uint32_t*>((uint8_t*)a.m + s0 + q * 128) = encode<true>(m[q], mi, rr, mtop);
+      *reinterpret_cast<uint32_t*>((uint8_t*)a.v + s0 + q * 128) = encode<false>(v[q], vi, rr, vtop);
+    }
+    if constexpr (AVERAGE) {
+      float e[4] = {x.e[q].x, x.e[q].y, x.e[q].z, x.e[q].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) e[i] = __fadd_rn(__fmul_rn(e[i], a.avg), __fmul_rn(w[q][i], a.avg1));
+      *reinterpret_cast<float4*>(a.average + s0 + q * 128) = make_float4(e[0], e[1], e[2], e[3]);
+    }
+  }
+}
+
+// Blocks per multiprocessor.  32-bit states are bound by memory: the next turn's values are on their way
+// while one is worked on (160 M values, 16 turns: 683 us, 100% of the copy rate; one turn per block 718 us).
+// 8-bit ones are bound by instructions: five blocks hold their values without spills (4: 585, 5: 539, 7: 613 us).
+constexpr int kResident32 = 4, kResident8 = 5;
+template <int BITS, bool AVERAGE>
+__global__ void __launch_bounds__(kThreads, BITS == 8 ? kResident8 : kResident32)
+adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
   __shared__ int s_last;
   const int4 c = a.chunks_n ? a.chunks[a.chunk0 + blockIdx.x] : make_int4(a.tensor0, 0, 0, 0);
   const Tensor tensor = list.t[c.x - a.tensor0];
   const bool skip = a.use_norm && a.ws->skip;
-  const bool active = tensor.grad != nullptr && !skip;
-  if (active) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int turns = 1 << a.shift, begin = warp * turns * kBlockValues;      // a warp's scale blocks are neighbours
+  if (tensor.grad != nullptr && !skip && begin < c.y) {
+    const int at = begin + lane * 4;     // quads at `at` and at + 128 of a turn
+    float* w = tensor.weight + (int64_t)c.w * a.chunk + at;
+    const float* g = tensor.grad + (int64_t)c.w * a.chunk + at;
+    int64_t s0 = (int64_t)c.z * kBlockValues + at;     // place in the state arrays
+    const bool wal = aligned16(w), gal = aligned16(g);
+    const int whole = c.y / kBlockValues * kBlockValues;      // scale blocks without values to leave out
+    const int mine = min(turns, (c.y - begin + kBlockValues - 1) / kBlockValues);
+    int from = begin;
+    Turn<BITS, AVERAGE> x;
+    read(x, a, w, g, s0, c.y - at, wal && gal && from < whole, wal, gal);
+    // Scale bytes are read and written once per warp, lane k that of turn k: a byte stored next to one
+    // that is read soon holds that read up (four turns with a byte each: 1,421 us, together: 591 us)
+    const int64_t scales = (int64_t)c.z + warp * turns + lane;
+    uint32_t ms = 1, vs = 1;
+    if (BITS == 8 && lane < mine) {
+      ms = a.m_scale[scales];
+      vs = a.v_scale[scales];
+    }
     const int64_t t = a.steps[c.x] + 1;
     Rate rate = a.rates[c.x];
-    float clip = 1.f;
-    if (a.use_norm) clip = a.ws->clip;
-    float* wp = tensor.weight + (int64_t)c.w * kChunk;
-    const float* gp = tensor.grad + (int64_t)c.w * kChunk;
-    const bool wal = aligned16(wp), gal = aligned16(gp);
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int at0 = warp * kBlockValues + lane * 4;     // quads at at0 and at0 + 128
-    const int64_t block = (int64_t)c.z + warp;          // scale block
-    const int64_t s0 = block * kBlockValues + lane * 4; // place in the state arrays
-    const bool used = warp * kBlockValues < c.y;        // this warp has values
-    float w[kQuads][4], g[kQuads][4], m[kQuads][4], v[kQuads][4];
-    if (used) {
-      float ms = 0.f, vs = 0.f;
+    const float clip = a.use_norm ? a.ws->clip : 1.f;
+    if (rate.t != t || rate.b1 != a.b1 || rate.b2 != a.b2) rate = rate_of(t, a.log_b1, a.log_b2, a.b1, a.b2);
+    const float size = a.lr * rate.m;
+#pragma unroll 1
+    for (int k = 0; k < mine; ++k) {
+      const bool fast = wal && gal && from < whole, next = wal && gal && from + kBlockValues < whole;
+      const int left = c.y - from - lane * 4;
+      constexpr bool PREFETCH = BITS == 32;
+      Turn<BITS, AVERAGE> y;
+      if (PREFETCH && k + 1 < mine)
+        read(y, a, w + kBlockValues, g + kBlockValues, s0 + kBlockValues, left - kBlockValues, next, wal, gal);
+      uint32_t mb = 0, vb = 0;
       if constexpr (BITS == 8) {
-        ms = __uint_as_float((uint32_t)a.m_scale[block] << 23);
-        vs = __uint_as_float((uint32_t)a.v_scale[block] << 23);
+        mb = __shfl_sync(0xffffffffu, ms, k);
+        vb = __shfl_sync(0xffffffffu, vs, k);
       }
-#pragma unroll
-      for (int q = 0; q < kQuads; ++q) {
-        const int at = at0 + q * 128;
-        const float4 gv = load4(gp + at, c.y - at, gal), wv = load4(wp + at, c.y - at, wal);
-        g[q][0] = gv.x; g[q][1] = gv.y; g[q][2] = gv.z; g[q][3] = gv.w;
-        w[q][0] = wv.x; w[q][1] = wv.y; w[q][2] = wv.z; w[q][3] = wv.w;
-        if constexpr (BITS == 32) {
-          const float4 mv = *reinterpret_cast<const float4*>((const float*)a.m + s0 + q * 128);
-          const float4 vv = *reinterpret_cast<const float4*>((const float*)a.v + s0 + q * 128);
-          m[q][0] = mv.x; m[q][1] = mv.y; m[q][2] = mv.z; m[q][3] = mv.w;
-          v[q][0] = vv.x; v[q][1] = vv.y; v[q][2] = vv.z; v[q][3] = vv.w;
-        } else {
-          const uint32_t mc = *reinterpret_cast<const uint32_t*>((const uint8_t*)a.m + s0 + q * 128);
-          const uint32_t vc = *reinterpret_cast<const uint32_t*>((const uint8_t*)a.v + s0 + q * 128);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            m[q][i] = decode<true>(mc, i, ms);
-            v[q][i] = decode<false>(vc, i, vs);
-          }
-        }
+      update(x, a, w, s0, left, fast, wal, clip, size, rate.v, t, mb, vb);
+      if (BITS == 8 && lane == k) {
+        ms = mb;
+        vs = vb;
       }
+      w += kBlockValues;
+      g += kBlockValues;
+      s0 += kBlockValues;
+      from += kBlockValues;
+      if constexpr (PREFETCH) x = y;
+      else if (k + 1 < mine) read(x, a, w, g, s0, left - kBlockValues, next, wal, gal);
     }
-    if (used) {
-      if (rate.t != t || rate.b1 != a.b1 || rate.b2 != a.b2) rate = rate_of(t, a.log_b1, a.log_b2, a.b1, a.b2);
-      const float size = a.lr * rate.m;
-      uint32_t mmax = 0, vmax = 0;      // as patterns: infinities and NaN are the largest
-#pragma unroll
-      for (int q = 0; q < kQuads; ++q) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float x = __fmul_rn(g[q][i], clip);
-          m[q][i] = __fadd_rn(__fmul_rn(m[q][i], a.b1), __fmul_rn(x, a.c1));
-          v[q][i] = __fadd_rn(__fmul_rn(v[q][i], a.b2), __fmul_rn(__fmul_rn(x, x), a.c2));
-          if constexpr (BITS == 8) {
-            mmax = max(mmax, __float_as_uint(fabsf(m[q][i])));
-            vmax = max(vmax, __float_as_uint(v[q][i]));      // a NaN of a sum of squares is positive
-            // bound by its instructions: hardware root and quotient (within 2 units in the last place)
-            float root;
-            asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v[q][i]));
-            const float den = fmaf(root, rate.v, a.eps);
-            w[q][i] = fmaf(w[q][i], a.keep, -size * __fdividef(m[q][i], den));
-          } else {
-            const float den = __fadd_rn(__fmul_rn(__fsqrt_rn(v[q][i]), rate.v), a.eps);
-            w[q][i] = __fsub_rn(__fmul_rn(w[q][i], a.keep), __fmul_rn(size, __fdiv_rn(m[q][i], den)));
-          }
-        }
-      }
-      bool write = true, mtop = false, vtop = false;
-      float mi = 0.f, vi = 0.f;
-      if constexpr (BITS == 8) {
-        mmax = __reduce_max_sync(0xffffffffu, mmax);
-        vmax = __reduce_max_sync(0xffffffffu, vmax);
-        write = max(mmax, vmax) < 0x7f800000u;
-        const uint32_t mb = scale_byte(mmax), vb = scale_byte(vmax);
-        mtop = mb == 253u;
-        vtop = vb == 253u;
-        mi = __uint_as_float((254u - mb) << 23);
-        vi = __uint_as_float((254u - vb) << 23);
-        if (write && lane == 0) {
-          a.m_scale[block] = (uint8_t)mb;
-          a.v_scale[block] = (uint8_t)vb;
-        }
-      }
-      if (write) {
-#pragma unroll
-        for (int q = 0; q < kQuads; ++q) {
-          const int at = at0 + q * 128;
-          store4(wp + at, w[q], c.y - at, wal);
-          if constexpr (BITS == 32) {
-            *reinterpret_cast<float4*>((float*)a.m + s0 + q * 128) = make_float4(m[q][0], m[q][1], m[q][2], m[q][3]);
-            *reinterpret_cast<float4*>((float*)a.v + s0 + q * 128) = make_float4(v[q][0], v[q][1], v[q][2], v[q][3]);
-          } else {
-            const uint64_t quad = (uint64_t)(s0 + q * 128) >> 2;
-            const uint4 r = philox(make_uint4((uint32_t)quad, (uint32_t)(quad >> 32), (uint32_t)t,
-                                              (uint32_t)((uint64_t)t >> 32)), a.keys);
-            const uint32_t rr[4] = {r.x, r.y, r.z, r.w};
-            const uint32_t mc = encode<true>(m[q], mi, rr, mtop), vc = encode<false>(v[q], vi, rr, vtop);
-            *reinterpret_cast<uint32_t*>((uint8_t*)a.m + s0 + q * 128) = mc;
-            *reinterpret_cast<uint32_t*>((uint8_t*)a.v + s0 + q * 128) = vc;
-          }
-          if constexpr (AVERAGE) {
-            float* ap = a.average + s0 + q * 128;   // padded: whole quads
-            const float4 av = *reinterpret_cast<const float4*>(ap);
-            float e[4] = {av.x, av.y, av.z, av.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) e[i] = __fadd_rn(__fmul_rn(e[i], a.avg), __fmul_rn(w[q][i], a.avg1));
-            *reinterpret_cast<float4*>(ap) = make_float4(e[0], e[1], e[2], e[3]);
-          }
-        }
-      }
+    if (BITS == 8 && lane < mine) {
+      a.m_scale[scales] = (uint8_t)ms;
+      a.v_scale[scales] = (uint8_t)vs;
     }
   }
   // The last block to finish advances the counters: every block has read its own by then.
@@ -451,8 +510,8 @@ int invalid(const char* what) {
 }
 
 bool bad_list(void* const* weights, const void* const* grads, int first_tensor, int tensors, const int32_t* chunks,
-              const int64_t* first_chunk, const void* workspace, bool need_weights) {
-  return tensors < 0 || first_tensor < 0 || !first_chunk || !workspace ||
+              const int64_t* first_chunk, int chunk, const void* workspace, bool need_weights) {
+  return tensors < 0 || first_tensor < 0 || !first_chunk || !workspace || chunk < kTurn || chunk > 32 * kTurn || (chunk & (chunk - 1)) ||
          (tensors > 0 && (!grads || !chunks || (need_weights && !weights)));
 }
 
@@ -461,19 +520,21 @@ bool bad_list(void* const* weights, const void* const* grads, int first_tensor, 
 
 using namespace ictc;
 
-extern "C" int ictc_adamw_chunk_values(void) { return kChunk; }
+extern "C" int ictc_adamw_turn_values(void) { return kTurn; }
 
 extern "C" int64_t ictc_adamw_workspace_bytes(void) { return (int64_t)sizeof(Workspace); }
 
 extern "C" int ictc_adamw_grad_norm(const void* const* grads, int tensors, const int32_t* chunks,
-                                    const int64_t* first_chunk, float max_norm, int clip, int skip_nonfinite,
+                                    const int64_t* first_chunk, int chunk, float max_norm, int clip, int skip_nonfinite,
                                     void* workspace, void* stream) {
-  if (bad_list(nullptr, grads, 0, tensors, chunks, first_chunk, workspace, false) || (clip && !(max_norm > 0.f)))
+  if (bad_list(nullptr, grads, 0, tensors, chunks, first_chunk, chunk, workspace, false) || (clip && !(max_norm > 0.f)))
     return invalid("ictc_adamw_grad_norm: invalid argument%s");
   const int launches = tensors ? (tensors + kList - 1) / kList : 1;
   if (launches > kNormBlocks) return invalid("ictc_adamw_grad_norm: too many tensors%s");
   Args a{};
   a.chunks = reinterpret_cast<const int4*>(chunks);
+  a.chunk = chunk;
+  while (kTurn << a.shift < chunk) ++a.shift;
   a.ws = static_cast<Workspace*>(workspace);
   const int cap = kNormBlocks / launches;
   int slot = 0;
@@ -484,7 +545,7 @@ extern "C" int ictc_adamw_grad_norm(const void* const* grads, int tensors, const
     for (int i = 0; i < a.tensors; ++i) list.t[i].grad = static_cast<const float*>(grads[a.tensor0 + i]);
     a.chunk0 = first_chunk[a.tensor0];
     a.chunks_n = first_chunk[a.tensor0 + a.tensors] - a.chunk0;
-    const int64_t want = a.chunks_n > 0 ? a.chunks_n : 1;
+    const int64_t turns = a.chunks_n << a.shift, want = turns > 0 ? turns : 1;
     const int grid = (int)(want < cap ? want : cap);
     const int last = k == launches - 1;
     grad_norm_kernel<<<grid, kThreads, 0, (cudaStream_t)stream>>>(list, a, slot, slot + grid, last, max_norm, clip,
@@ -496,16 +557,18 @@ extern "C" int ictc_adamw_grad_norm(const void* const* grads, int tensors, const
 }
 
 extern "C" int ictc_adamw_step(void* const* weights, const void* const* grads, int first_tensor, int tensors,
-                               const int32_t* chunks, const int64_t* first_chunk, int bits, void* m, void* v,
+                               const int32_t* chunks, const int64_t* first_chunk, int chunk, int bits, void* m, void* v,
                                uint8_t* m_scale, uint8_t* v_scale, float* average, int64_t* steps, void* rates, double lr,
                                double beta1, double beta2, double eps, double weight_decay, double average_decay,
                                uint64_t seed, int use_norm, void* workspace, void* stream) {
-  if (bad_list(weights, grads, first_tensor, tensors, chunks, first_chunk, workspace, true) ||
+  if (bad_list(weights, grads, first_tensor, tensors, chunks, first_chunk, chunk, workspace, true) ||
       (bits != 8 && bits != 32) || !(beta1 >= 0.0 && beta1 < 1.0) || !(beta2 >= 0.0 && beta2 < 1.0) ||
       !((float)eps > 0.f) || (tensors > 0 && (!steps || !rates || !m || !v || (bits == 8 && (!m_scale || !v_scale)))))
     return invalid("ictc_adamw_step: invalid argument%s");
   Args a{};
   a.chunks = reinterpret_cast<const int4*>(chunks);
+  a.chunk = chunk;
+  while (kTurn << a.shift < chunk) ++a.shift;
   a.m = m;
   a.v = v;
   a.m_scale = m_scale;

@@ -60,10 +60,10 @@ _SIGNATURES = {
     "ictc_radial_pack": [_p, _p, _p, _p, _i, _i, _i, _p, _i64],
     "ictc_radial_forward": [_p, _p, _p, _i64, _i, _i, _i, _p, _p],
     "ictc_radial_backward": [_p, _p, _p, _p, _p, _i64, _i, _i, _i, _p, _p],
-    "ictc_adamw_chunk_values": [],
+    "ictc_adamw_turn_values": [],
     "ictc_adamw_workspace_bytes": [],
-    "ictc_adamw_grad_norm": [_p, _i, _p, _p, _f, _i, _i, _p, _p],
-    "ictc_adamw_step": [_p, _p, _i, _i, _p, _p, _i, _p, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _d, _u64, _i, _p,
+    "ictc_adamw_grad_norm": [_p, _i, _p, _p, _i, _f, _i, _i, _p, _p],
+    "ictc_adamw_step": [_p, _p, _i, _i, _p, _p, _i, _i, _p, _p, _p, _p, _p, _p, _p, _d, _d, _d, _d, _d, _d, _u64, _i, _p,
                         _p],
     "ictc_block_partial_floats": [_i, _i],
     "ictc_block_supported": [_i, _i],

@@ -14,18 +14,35 @@ from . import _native
 from ._native import launch
 
 BLOCK = 256   # values that share a scale of the 8-bit moments (csrc/adamw.cu)
+WAVE = 740    # blocks that a B200 holds at once
 
 
 def blocks_of(numel: int) -> int:
     return -(-numel // BLOCK)
 
 
+def turns_of(total: int) -> int:
+    """Turns of 1,024 values per block: as many as leave one wave of blocks, 8 at most.
+
+    Microseconds of a step with 32 / 8-bit states and 1, 2, 4, 8, 16 turns:
+    30,000 values 8.3 10.1 10.3 13.3 19.2 / 6.2 8.3 10.3 12.4 18.5;  1 M 12.4 10.3 12.1 14.4 20.9 / 11.0
+    10.3 10.3 14.4 20.5;  4 M 24.9 20.4 20.2 18.5 22.6 / 24.8 20.6 20.4 20.7 24.4;  16 M 95 79 77 76 78 / 91
+    74 67 66 74;  160 M 879 689 664 674 678 / 843 656 580 538 529."""
+    turns = 1
+    while turns < 8 and total > turns * 1024 * WAVE:
+        turns *= 2
+    return turns
+
+
 class TensorTable:
     """Chunks and state places of tensors of the given sizes."""
 
-    def __init__(self, sizes, device):
-        chunk = int(_native.library().ictc_adamw_chunk_values())
-        sizes = torch.tensor(list(sizes), dtype=torch.int64)
+    def __init__(self, sizes, device, turns=None):
+        sizes = list(sizes)
+        if turns is None:
+            turns = turns_of(sum(sizes))
+        chunk = turns * int(_native.library().ictc_adamw_turn_values())
+        sizes = torch.tensor(sizes, dtype=torch.int64)
         blocks = (sizes + BLOCK - 1) // BLOCK
         counts = (sizes + chunk - 1) // chunk
         first = torch.zeros(sizes.numel() + 1, dtype=torch.int64)
@@ -38,7 +55,7 @@ class TensorTable:
         values = torch.clamp(sizes[tensor] - number * chunk, max=chunk)
         block = starts[tensor] + number * (chunk // BLOCK)
         table = torch.stack((tensor, values, block, number), 1).to(torch.int32)
-        self.count = sizes.numel()
+        self.count, self.chunk = sizes.numel(), chunk
         self.starts = (starts * BLOCK).tolist()
         self.blocks = int(blocks.sum())
         self.values = self.blocks * BLOCK
@@ -52,11 +69,11 @@ class TensorTable:
     def grad_norm(self, grads, max_norm, skip_nonfinite):
         """``grads``: address of a host array of ``count`` device pointers (0: no gradient)."""
         launch(self.chunks.device, "ictc_adamw_grad_norm", grads, self.count, self.chunks, self.first_chunk,
-               1.0 if max_norm is None else max_norm, max_norm is not None, skip_nonfinite, self.workspace)
+               self.chunk, 1.0 if max_norm is None else max_norm, max_norm is not None, skip_nonfinite, self.workspace)
 
     def step(self, weights, grads, first, count, bits, state, *, lr, betas, eps, weight_decay, ema_decay, seed,
              use_norm):
-        launch(self.chunks.device, "ictc_adamw_step", weights, grads, first, count, self.chunks, self.first_chunk, bits,
+        launch(self.chunks.device, "ictc_adamw_step", weights, grads, first, count, self.chunks, self.first_chunk, self.chunk, bits,
                state["m"], state["v"], state["m_scale"], state["v_scale"], state["average"], state["steps"], state["rates"], lr,
                betas[0], betas[1], eps, weight_decay, ema_decay, seed, use_norm, self.workspace)
 

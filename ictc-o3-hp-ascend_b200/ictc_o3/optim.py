@@ -223,7 +223,7 @@ class AdamW(torch.optim.Optimizer):
             values["lr"] = float(values["lr"])
             _hyperparameters(values)
             loaded.append(values)
-        names = [name for group in groups for name in group["params"]]
+        names, exponents = [name for group in groups for name in group["params"]], []
         for name, p in zip(names, self._params):
             entry, mine = saved.get(name), self.state[p]
             if entry is None:
@@ -239,8 +239,10 @@ class AdamW(torch.optim.Optimizer):
                         raise ValueError("a step count is negative")
                 elif not isinstance(theirs, torch.Tensor) or theirs.dtype != value.dtype or theirs.shape != value.shape:
                     raise ValueError(f"{key} has another type or shape; was it saved with other state_bits?")
-                elif key.endswith("exponent") and theirs.numel() and (int(theirs.min()) < 1 or int(theirs.max()) > 253):
-                    raise ValueError(f"{key} is outside 1..253")
+                elif key.endswith("exponent") and theirs.numel():
+                    exponents.append(theirs.to(self._device))
+        if exponents and not 1 <= int((all_of := torch.cat(exponents)).min()) <= int(all_of.max()) <= 253:
+            raise ValueError("a scale exponent is outside 1..253")
         for group, values in zip(self.param_groups, loaded):
             group.update(values, betas=tuple(values["betas"]))
         steps, to, values = [], [], []

@@ -356,7 +356,8 @@ int ictc_neighbor_list_noalloc(const float* pos, int64_t atoms, const float* box
  *
  * Static tables, built once by the caller:
  *   chunks       device int32 [n][4]: every tensor is cut into chunks of
- *                ictc_adamw_chunk_values() consecutive values (the last one shorter);
+ *                `chunk` consecutive values (the last one shorter), a multiple of
+ *                ictc_adamw_turn_values();
  *                {tensor, values in the chunk, first 256-value block of the chunk in
  *                the state arrays, number of the chunk inside its tensor}
  *   first_chunk  host int64 [tensors + 1]: first chunk of every tensor
@@ -379,12 +380,12 @@ int ictc_neighbor_list_noalloc(const float* pos, int64_t atoms, const float* box
  * ictc_adamw_grad_norm found.  With bits = 8 a 256-value block whose new moments are
  * not finite is left as it was.
  */
-int ictc_adamw_chunk_values(void);
+int ictc_adamw_turn_values(void);
 int64_t ictc_adamw_workspace_bytes(void);
 int ictc_adamw_grad_norm(const void* const* grads, int tensors, const int32_t* chunks, const int64_t* first_chunk,
-                         float max_norm, int clip, int skip_nonfinite, void* workspace, void* stream);
+                         int chunk, float max_norm, int clip, int skip_nonfinite, void* workspace, void* stream);
 int ictc_adamw_step(void* const* weights, const void* const* grads, int first_tensor, int tensors,
-                    const int32_t* chunks, const int64_t* first_chunk, int bits, void* m, void* v, uint8_t* m_scale,
+                    const int32_t* chunks, const int64_t* first_chunk, int chunk, int bits, void* m, void* v, uint8_t* m_scale,
                     uint8_t* v_scale, float* average, int64_t* steps, void* rates, double lr, double beta1,
                     double beta2, double eps, double weight_decay, double average_decay, uint64_t seed, int use_norm,
                     void* workspace, void* stream);

@@ -7,13 +7,15 @@ import torch
 from oracle import adamw_oracle
 
 
-def test_chunk_table_covers_every_value_once():
+@pytest.mark.parametrize("turns", [1, 4])
+def test_chunk_table_covers_every_value_once(turns):
     from ictc_o3.backends.cuda import _native
     from ictc_o3.backends.cuda.adamw import TensorTable
-    chunk = int(_native.library().ictc_adamw_chunk_values())
+    chunk = turns * int(_native.library().ictc_adamw_turn_values())
     sizes = [1, chunk, chunk + 1, 0, 255, 256, 257, 5 * chunk - 3, 3]
-    table = TensorTable(sizes, "cpu")
+    table = TensorTable(sizes, "cpu", turns)
     rows = table.chunks.tolist()
+    assert table.chunk == chunk
     assert list(table.first_chunk) == [0, 1, 2, 4, 4, 5, 6, 7, 12, 13]
     assert table.starts == [0, 256, 256 + chunk, 2 * chunk + 512] + [
         2 * chunk + 512 + d for d in (0, 256, 512, 1024, 1024 + 5 * chunk)]
@@ -23,6 +25,11 @@ def test_chunk_table_covers_every_value_once():
         assert [r[3] for r in mine] == list(range(len(mine)))
         assert [256 * r[2] for r in mine] == [table.starts[t] + k * chunk for k in range(len(mine))]
     assert table.values == table.starts[-1] + 256 and table.values == 256 * table.blocks
+
+
+def test_turns_grow_with_the_total():
+    from ictc_o3.backends.cuda.adamw import turns_of
+    assert [turns_of(n) for n in (1, 700_000, 1_000_000, 3_000_000, 20_000_000, 10 ** 10)] == [1, 1, 2, 4, 8, 8]
 
 
 def test_state_format_is_monotone_and_round_trips():
@@ -70,23 +77,24 @@ def test_native_entry_points_validate_before_launching():
     first = (ctypes.c_int64 * 2)(0, 1)
     ones = (ctypes.c_void_p * 1)(1)
     some = ctypes.c_void_p(1)
-    common = [first, 32, some, some, None, None, None, some, some, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 0]
+    common = [first, 1024, 32, some, some, None, None, None, some, some, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0, 0, 0]
 
     def step(**change):
-        names = ["first_chunk", "bits", "m", "v", "m_scale", "v_scale", "average", "steps", "rates", "lr", "b1", "b2", "eps",
+        names = ["first_chunk", "chunk", "bits", "m", "v", "m_scale", "v_scale", "average", "steps", "rates", "lr", "b1", "b2", "eps",
                  "wd", "avg", "seed", "use_norm"]
         values = dict(zip(names, common), **change)
         return lib.ictc_adamw_step(change.pop("weights", ones), ones, 0, 1, some, *[values[n] for n in names], some,
                                    None)
 
     for change in ({"bits": 16}, {"bits": 8}, {"m": None}, {"steps": None}, {"rates": None}, {"b1": 1.0}, {"b2": -0.1}, {"eps": 0.0},
-                   {"eps": 1e-50}, {"first_chunk": None}):
+                   {"eps": 1e-50}, {"first_chunk": None},
+                   {"chunk": 0}, {"chunk": 1000}, {"chunk": 1536}, {"chunk": 1 << 20}):
         assert step(**change) == -1, change
         assert "invalid" in lib.ictc_last_error().decode()
     assert lib.ictc_adamw_step(ones, ones, 0, -1, some, *common, some, None) == -1
     assert lib.ictc_adamw_step(ones, ones, 0, 1, some, *common, None, None) == -1
-    assert lib.ictc_adamw_grad_norm(ones, 1, some, first, 0.0, 1, 0, some, None) == -1
-    assert lib.ictc_adamw_grad_norm(None, 1, some, first, 1.0, 1, 0, some, None) == -1
+    assert lib.ictc_adamw_grad_norm(ones, 1, some, first, 1024, 0.0, 1, 0, some, None) == -1
+    assert lib.ictc_adamw_grad_norm(None, 1, some, first, 1024, 1.0, 1, 0, some, None) == -1
     assert lib.ictc_adamw_decode(some, some, some, some, 255, some, some, None) == -1
     assert lib.ictc_adamw_decode(None, None, None, None, 256, None, None, None) == -1
     assert lib.ictc_adamw_decode(None, None, None, None, 0, None, None, None) == 0

@@ -10,7 +10,7 @@ pytestmark = pytest.mark.gpu
 
 HYPER = {"lr": 3e-3, "betas": (0.9, 0.99), "eps": 1e-8, "weight_decay": 0.02}
 SIZES = {"one": [1], "edges": [3, 4, 5, 255, 256, 257, 2047, 2048, 2049, 1], "empty": [0, 7, 0, 1025],
-         "many": [1 + 37 * k % 911 for k in range(500)], "large": [1_300_003]}
+         "many": [1 + 37 * k % 911 for k in range(500)], "large": [1_300_003], "turns": [3_100_001, 9000, 40_000, 255, 3_000_000]}
 
 
 def make(sizes, device, seed=0, offset=0):
@@ -97,12 +97,15 @@ def test_32_bit_step_against_fp64(name, offset, ema, clip, cuda_device):
 
 
 @pytest.mark.parametrize("name", list(SIZES))
-def test_8_bit_codes_are_exact(name, cuda_device):
+def test_8_bit_codes_are_exact(name, cuda_device, monkeypatch):
     """Without clipping every operation before the rounding is a single FP32 operation, so the codes
     equal those of the FP32 restatement; weights meet the FP32 bounds."""
     from ictc_o3.optim import AdamW
-    sizes = SIZES[name] if name != "large" else [200_003]
+    sizes = {"large": [200_003], "turns": [9001, 70_000]}.get(name, SIZES[name])
     params = make(sizes, cuda_device, seed=3, offset=1 if name == "edges" else 0)
+    if name == "turns":      # blocks of several turns, as many values have them
+        from ictc_o3.backends.cuda import adamw
+        monkeypatch.setattr(adamw, "turns_of", lambda total: 8)
     opt = AdamW(params, **HYPER, state_bits=8, seed=0x0123456789ABCDEF)
     before = random_state(opt, 2)
     old = [p.detach().double() for p in params]
