@@ -62,7 +62,7 @@ bool shape_of(int C, int L, int mode, unsigned there, bool sums, int64_t rows, i
   if (wanted < most) most = (int)(wanted > 0 ? wanted : 1);
   for (s->stages = 4; s->stages >= 1; --s->stages) {
     const int64_t bytes = 4 * (s->stages * stage + fixed);
-    int64_t groups = (s->stages > 1 ? kSharedBudget : kSharedLimit) / bytes;
+    int64_t groups = (s->stages > 1 ? shared_budget(mode) : kSharedLimit) / bytes;
     if (groups > most) groups = most;
     // fewer stages where they make room for more groups, two where two fit
     if (groups < 1 || (groups < most && s->stages > 2)) {

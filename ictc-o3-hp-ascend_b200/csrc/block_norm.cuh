@@ -49,9 +49,11 @@ namespace block_norm {
 constexpr int kMaxL = 3;
 constexpr int kMaxDevices = 64;
 constexpr int kSharedLimit = 227 * 1024;
-constexpr int kSharedBudget = 220 * 1024;
 
 enum Mode : int { kForward = 0, kBackward = 1, kSecond = 2 };
+
+// Of 227 KB; the forward does better with some left as L1 (32,768 rows of C128/lmax 3: 196 us with 220 KB).
+__host__ __device__ constexpr int shared_budget(int mode) { return (mode == kForward ? 200 : 220) * 1024; }
 
 // Staged tensors: 0..5 rows, then per-channel and per-degree ones.
 //   forward  y h . . . .      backward  y h' p q . .      second  y h' p q al be
@@ -61,24 +63,28 @@ enum Slot : int { kY, kH, kP, kQ, kAl, kBe, kGate, kGateDot, kR1, kR2, kSlots };
 // Rows that a lane works on at once, and warps per block, by mode and lmax.  Low degrees have few
 // values per row: several rows share a tile's barriers, sums and copies.  More rows per lane mean
 // more registers and so fewer warps; measured on 50,000 to 100,000 rows, both sides of each choice:
-//   forward  lmax 0, C128: 8 rows 74 us, 4 rows 96;  lmax 1, C132: 4 rows 98, 2 rows 127
+//   forward  lmax 0, C128: 8 rows 74 us, 4 rows 96;  lmax 1, C132: 4 rows 98, 2 rows 127;
+//            lmax 2, 262,144 rows of C64: 2 rows 454 (20 warps), 1 row 437 (24 warps);  lmax 3, 32,768
+//            rows of C128: 20 warps 196, 16 warps 190
 //   backward lmax 0, C128: 8 rows 104, 4 rows 141;  lmax 1, C132: 4 rows 223 (16 warps), 2 rows 162 (20 warps);
 //            lmax 2, C64: 2 rows 217, 1 row 178;  lmax 3, 8,192 rows of C128: 16 warps 90, 12 warps 84
-//   second   lmax 0, C128: 4 rows 262 (12 warps), 1 row 315 (16 warps);  lmax 1, C50: 2 rows 133, 1 row 150;
-//            lmax 2, C64: 2 rows 487, 1 row 328
+//   second   lmax 0, C128: 4 rows 218 (16 warps) or 263 (12), 2 rows 347;  lmax 1, C50: 2 rows 142, 1 row 171;
+//            lmax 2, C64: 2 rows 404, 1 row 331
 __host__ __device__ constexpr int rows_per_lane(int mode, int L, bool hold) {
-  constexpr int rows[3][kMaxL + 1] = {{8, 4, 2, 1}, {8, 2, 1, 1}, {4, 2, 1, 1}};
+  constexpr int rows[3][kMaxL + 1] = {{8, 4, 1, 1}, {8, 2, 1, 1}, {4, 2, 1, 1}};
   return hold ? rows[mode][L] : 1;
 }
 __host__ __device__ constexpr int max_warps(int mode, int L) {
-  constexpr int warps[3][kMaxL + 1] = {{24, 24, 20, 20}, {16, 20, 20, 12}, {12, 12, 12, 8}};
+  constexpr int warps[3][kMaxL + 1] = {{24, 24, 24, 16}, {16, 20, 20, 12}, {16, 12, 12, 8}};
   return warps[mode][L];
 }
-// Warps of one row at most; wider rows take turns (HOLD false).
+// Warps of one row at most; wider rows take turns (HOLD false), and the widest ones leave room
+// for the scratch of twelve.
 __host__ __device__ constexpr int max_row_warps(int mode, int L) {
-  return max_warps(mode, L) < 16 ? max_warps(mode, L) : 16;
+  const int most = mode == kSecond ? 12 : 16;
+  return max_warps(mode, L) < most ? max_warps(mode, L) : most;
 }
-constexpr int kScratch = 16;   // sums of one warp
+constexpr int kScratch = 16;                          // sums of one warp
 constexpr int kBarrierFloats = 8;                     // room of four mbarriers
 constexpr uint64_t kWaitNs = 2000000000ull;           // a copy that takes longer is given up
 
