@@ -32,6 +32,16 @@
 // block's lanes (HOLD false) go over their channels in turns and read shared memory again
 // in every phase.  Weight gradients are summed per block and then over blocks by a second kernel, in
 // a fixed order: no atomics, the same bits every time.
+//
+// Measured on a B200 (copy rate 6,565 GB/s; bytes: every row array once), with gate:
+//   262,144 rows of C64/lmax 2: forward 438 us (5,970 GB/s), backward with weights 653 us (6,160),
+//   second 1,265 us (5,250);  8,192 rows of C128/lmax 3: 53 us (5,360), 84 us (5,200), 176 us (4,100);
+//   100,000 rows of C128/lmax 0: 76 us (3,380), 104 us (3,920), 221 us (3,010).
+// The forward and the first gradients are near the memory's rate.  The second derivatives at lmax 3 stage 53 KB per
+// row of C128, so two rows are worked on and two are under way per multiprocessor: their eight warps wait on one
+// another's sums and on arrivals (issue slots 37% taken).  Two sets of warps per row, one for degree 3
+// and one for the rest, measured the same (177 us) and were dropped.  At lmax 0 a row is short and the fixed
+// work per tile (sums, barriers, copies) shows.
 #pragma once
 
 #include "ictc_common.cuh"
