@@ -340,7 +340,7 @@ __device__ __forceinline__ void update(const Turn<BITS, AVERAGE>& x, const Args&
         vmax = max(vmax, __float_as_uint(v[q][i]));      // a NaN of a sum of squares is positive
         // bound by its instructions: hardware root and quotient (within 2 units in the last place)
         float root;
-        asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(root) : "f"(v[q][i]));
+        asm("sqrt.approx.f32 %0, %1;" : "=f"(root) : "f"(v[q][i]));
         const float den = fmaf(root, rate, a.eps);
         w[q][i] = fmaf(ow[i], a.keep, -size * __fdividef(m[q][i], den));
       } else {

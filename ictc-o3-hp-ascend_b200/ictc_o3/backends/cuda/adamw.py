@@ -63,19 +63,21 @@ class TensorTable:
         self.first_chunk = (ctypes.c_int64 * (self.count + 1))(*first.tolist())
         self.workspace = torch.zeros(int(_native.library().ictc_adamw_workspace_bytes()), dtype=torch.uint8,
                                      device=device)
+        self.device, self.chunks_at, self.workspace_at = (self.workspace.device, self.chunks.data_ptr(),
+                                                          self.workspace.data_ptr())
         # word 2 of the workspace: gradient norm of the last step that computed one
         self.norm = self.workspace[8:12].view(torch.float32)[0]
 
     def grad_norm(self, grads, max_norm, skip_nonfinite):
         """``grads``: address of a host array of ``count`` device pointers (0: no gradient)."""
-        launch(self.chunks.device, "ictc_adamw_grad_norm", grads, self.count, self.chunks, self.first_chunk,
-               self.chunk, 1.0 if max_norm is None else max_norm, max_norm is not None, skip_nonfinite, self.workspace)
+        launch(self.device, "ictc_adamw_grad_norm", grads, self.count, self.chunks_at, self.first_chunk, self.chunk,
+               1.0 if max_norm is None else max_norm, max_norm is not None, skip_nonfinite, self.workspace_at)
 
     def step(self, weights, grads, first, count, bits, state, *, lr, betas, eps, weight_decay, ema_decay, seed,
              use_norm):
-        launch(self.chunks.device, "ictc_adamw_step", weights, grads, first, count, self.chunks, self.first_chunk, self.chunk, bits,
-               state["m"], state["v"], state["m_scale"], state["v_scale"], state["average"], state["steps"], state["rates"], lr,
-               betas[0], betas[1], eps, weight_decay, ema_decay, seed, use_norm, self.workspace)
+        """``state``: addresses of m, v, their scales, the average, steps and rates (this optimizer's own)."""
+        launch(self.device, "ictc_adamw_step", weights, grads, first, count, self.chunks_at, self.first_chunk, self.chunk,
+               bits, *state, lr, *betas, eps, weight_decay, ema_decay, seed, use_norm, self.workspace_at)
 
     def decode(self, state):
         """BF16 values of the 8-bit moments."""

@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import math
 from array import array
+from operator import attrgetter
 
 import torch
 
@@ -24,6 +25,17 @@ def _number(value, name, low, high=math.inf, open_low=False):
     if not (low < value if open_low else low <= value) or not value < high:
         raise ValueError(f"{name} is outside its range")
     return value
+
+
+# what a step needs to know of all its tensors: (FP32?, device, values, contiguous?), column by column
+_gradient, _dtype = attrgetter("grad"), attrgetter("dtype")
+_device, _numel = torch.Tensor.get_device, torch.Tensor.numel
+_contiguous, _address = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
+
+
+def _columns(tensors):
+    return (list(map(_dtype, tensors)), list(map(_device, tensors)), list(map(_numel, tensors)),
+            list(map(_contiguous, tensors)))
 
 
 def _hyperparameters(group):
@@ -120,7 +132,10 @@ class AdamW(torch.optim.Optimizer):
                     entry["ema"].copy_(p.detach())
                 self.state[p] = entry
         self._params, self._flat, self._device = params, flat, device
-        self._expected = [(torch.float32, device.index, p.numel(), True) for p in params]
+        self._places = [None if flat[k] is None else flat[k].data_ptr()
+                        for k in ("m", "v", "m_scale", "v_scale", "average", "steps", "rates")]
+        self._expected = ([torch.float32] * len(params), [device.index] * len(params), [p.numel() for p in params],
+                          [True] * len(params))
         self._full = all(p.numel() for p in params)
         self._table = table
         self._empty = table.workspace.data_ptr()      # stands for the gradient of a tensor without values
@@ -134,27 +149,28 @@ class AdamW(torch.optim.Optimizer):
         """Addresses of weights and gradients (0: no gradient), the updated weights, and
         temporaries that must outlive the launch."""
         params, expected = self._params, self._expected
-        grads = [p.grad for p in params]
+        grads = list(map(_gradient, params))
         live, kept = params, ()
-        try:      # as a rule: a dense, contiguous gradient everywhere, found by one comparison
-            fine = [(g.dtype, g.get_device(), g.numel(), g.is_contiguous()) for g in grads] == expected
-            places = [g.data_ptr() for g in grads] if fine else None
-        except (AttributeError, RuntimeError):      # None, or a layout without an address
+        try:      # as a rule: a dense, contiguous gradient everywhere
+            fine = _columns(grads) == expected
+            places = list(map(_address, grads)) if fine else None
+        except (AttributeError, TypeError, RuntimeError):      # None, or a layout without an address
             fine = False
         if not fine:
-            live = [p for p, g in zip(params, grads) if g is not None]
-            expected = [e for e, g in zip(expected, grads) if g is not None]
-        if [(p.dtype, p.get_device(), p.numel(), p.is_contiguous()) for p in live] != expected:
+            there = [g is not None for g in grads]
+            live = [p for p, t in zip(params, there) if t]
+            expected = tuple([e for e, t in zip(column, there) if t] for column in expected)
+        if _columns(live) != expected:
             raise ValueError("a parameter has changed its type, device, size or layout since the optimizer was built")
         if not fine:
-            for g, e in zip([g for g in grads if g is not None], expected):
-                if g.layout is not torch.strided or (g.dtype, g.get_device(), g.numel()) != e[:3]:
-                    raise ValueError("gradients must be dense CUDA FP32 tensors of their parameter's size")
+            given = [g for g in grads if g is not None]
+            if any(g.layout is not torch.strided for g in given) or _columns(given)[:3] != expected[:3]:
+                raise ValueError("gradients must be dense CUDA FP32 tensors of their parameter's size")
             kept = [None if g is None else g.detach().contiguous() for g in grads]
             places = [0 if g is None else g.data_ptr() for g in kept]
         if not self._full:      # a tensor without values has no address, but its steps count
             places = [self._empty if g is not None and not g.numel() else k for g, k in zip(grads, places)]
-        return array("Q", [p.data_ptr() for p in params]), array("Q", places), live, kept
+        return array("Q", list(map(_address, params))), array("Q", places), live, kept
 
     def step(self, closure=None):
         loss = None
@@ -172,7 +188,7 @@ class AdamW(torch.optim.Optimizer):
         first = 0
         for group, values in zip(self.param_groups, groups):
             count = len(group["params"])
-            self._table.step(w, g, first, count, self.state_bits, self._flat, **values,
+            self._table.step(w, g, first, count, self.state_bits, self._places, **values,
                              ema_decay=0.0 if self.ema_decay is None else self.ema_decay, seed=self.seed,
                              use_norm=use_norm)
             first += count
@@ -243,8 +259,10 @@ class AdamW(torch.optim.Optimizer):
                     exponents.append(theirs.to(self._device))
         if exponents and not 1 <= int((all_of := torch.cat(exponents)).min()) <= int(all_of.max()) <= 253:
             raise ValueError("a scale exponent is outside 1..253")
-        for group, values in zip(self.param_groups, loaded):
-            group.update(values, betas=tuple(values["betas"]))
+        for group, theirs, values in zip(self.param_groups, groups, loaded):
+            # other entries (a scheduler's initial_lr) come along
+            group.update({k: v for k, v in theirs.items() if k != "params"}, **values)
+            group["betas"] = tuple(values["betas"])
         steps, to, values = [], [], []
         for name, p in zip(names, self._params):
             entry, mine = saved.get(name), self.state[p]

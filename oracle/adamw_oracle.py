@@ -31,8 +31,7 @@ def step_bounds(w, g, m, v, t, *, lr, betas, eps, weight_decay, clip=1.0, clippe
     m.  sqrt halves v's error; + 1 for itself, 1 for the constant 1/sqrt(1-b2^t), 1 for the
     product, 1 for + eps, 1 for eps itself.  The quotient 1, lr/(1-b1^t) 1, the product 1.
     ``approximate``: root and quotient by hardware approximations, each within 2 units in the last
-    place = 4 half steps instead of 1 (root's and denominator's flush of values below 2^-126 included
-    in eps: eps >= 2^-126 / U is assumed).
+    place = 4 half steps instead of 1.
     Weights: constant 1, product 1, difference 1."""
     b1, b2 = betas
     e = 5.0 if clipped else 0.0

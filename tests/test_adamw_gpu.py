@@ -277,6 +277,26 @@ def test_other_stream_and_strided_gradient(cuda_device):
     assert torch.equal(a, b)
 
 
+def test_tiny_gradients_and_epsilon(cuda_device):
+    """Second moments below FP32's normal range still divide (no flush to zero), in both forms."""
+    from ictc_o3.optim import AdamW
+    hyper = {**HYPER, "eps": 1e-24}
+    for bits in (32, 8):
+        p = torch.nn.Parameter(torch.randn(700, device=cuda_device))
+        p.grad = torch.randn(700, device=cuda_device) * 3e-20
+        w, g, zero = p.detach().double(), p.grad.double(), torch.zeros(700, dtype=torch.float64, device=cuda_device)
+        opt = AdamW([p], **hyper, state_bits=bits)
+        opt.step()
+        # v = (1 - b2) g^2 is some 1e-41, a multiple of 2^-149: its root is off by up to 2^-149 / (2 root), and the
+        # quotient, of size 1, by that over the root
+        v = 0.01 * g * g
+        want = adamw_oracle.step(w, g, zero, zero, 1, **hyper)[0]
+        loose = hyper["lr"] * 2.0 ** -149 / v.clamp_min(2.0 ** -149) * 2
+        fine = v > 64 * 2.0 ** -149
+        bound = adamw_oracle.step_bounds(w, g, zero, zero, 1, **hyper, approximate=bits == 8)[0] + loose
+        assert fine.sum() > 300 and bool(((p.detach().double() - want).abs() <= bound)[fine].all())
+
+
 def test_results_are_reproducible_and_seeded(cuda_device):
     from ictc_o3.optim import AdamW
 
@@ -339,6 +359,16 @@ def test_state_dicts(cuda_device):
     bad["state"][0]["exp_avg_exponent"][0] = 255
     with pytest.raises(ValueError, match="1..253"):
         opt.load_state_dict(bad)
+    # a scheduler continues where it was
+    first = AdamW(make([5], cuda_device), lr=1e-2)
+    schedule = torch.optim.lr_scheduler.StepLR(first, 1, 0.5)
+    first.step()
+    schedule.step()
+    second = AdamW(make([5], cuda_device), lr=1.0)
+    second.load_state_dict(first.state_dict())
+    assert second.param_groups[0]["initial_lr"] == 1e-2
+    torch.optim.lr_scheduler.StepLR(second, 1, 0.5, last_epoch=schedule.last_epoch).step()
+    assert second.param_groups[0]["lr"] < 5e-3 + 1e-9
     with pytest.raises(ValueError, match="parameter groups"):
         AdamW(make([700], cuda_device)).load_state_dict(opt.state_dict())
     # the library's own state continues here

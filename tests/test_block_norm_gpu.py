@@ -436,6 +436,26 @@ def test_streams_and_capture(cuda_device):
     assert all(torch.equal(a, b) for a, b in zip(held, fresh))
 
 
+def test_first_call_inside_a_capture(cuda_device, monkeypatch):
+    """Nothing that a first call sets up (status word, scratch size) needs to be there before a capture."""
+    from ictc_o3.backends.cuda import block_norm
+    from ictc_o3.ops.block_norm import block_norm_status, residual_block_norm
+    monkeypatch.setattr(block_norm, "_status", {})
+    monkeypatch.setattr(block_norm, "_partial_floats", {})
+    t = inputs(50, 20, 1)
+
+    def step():
+        out = residual_block_norm(t["stream"], t["branch"], scale=t["scale"], norm=True, channels=20, lmax=1)
+        return [x.detach() for x in (*out, *torch.autograd.grad(out, [t["branch"], t["scale"]], [t["p"], t["q"]]))]
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(held, step()))
+    assert block_norm_status() == 0
+
+
 def test_refusals(cuda_device):
     from ictc_o3.ops.block_norm import ResidualBlockNorm, degree_norm, residual_block_norm
     x = torch.zeros(4, 72, device=cuda_device)
