@@ -169,7 +169,9 @@ class _Block(torch.autograd.Function):
         if p is None and q is None:
             return (None,) * 7
         # asked of the engine: whether the branch's gradient runs (a row written or not) and whether any
-        # weight's does (forces need none); the weights share their sums, and a gate's gradient is small
+        # weight's does; the weights share their sums, and a gate's gradient is small.  autograd.grad does not tell
+        # for leaves, so a pass for forces sums the weights' gradients too (6 us at 8,192 rows of C128/lmax 3;
+        # views that could be asked cost 25 us of host time)
         _, need_stream, need_branch, need_gate, *need_weights = ctx.needs_input_grad
         nodes = iter([node for node, _ in ctx.next_functions])      # of the tensors among the arguments
         _, at_branch, _, *at_weights = [None if t is None else next(nodes) for t in ctx.saved_tensors]
@@ -231,9 +233,6 @@ def block(form, stream, branch, gate, post, scale, pre):
     """(stream', normed) of contiguous arguments; without anything to differentiate no graph is made."""
     args = (stream, branch, gate, post, scale, pre)
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args]):
-        # views of leaves: a pass for forces can tell that their gradients do not run
-        post, scale, pre = [w.view_as(w) if w is not None and w.requires_grad and w.is_leaf else w
-                            for w in (post, scale, pre)]
-        out = _Block.apply(form, stream, branch, gate, post, scale, pre)
+        out = _Block.apply(form, *args)
         return (None, out[0]) if branch is None else out if form.norm else (out[0], None)
     return _forward(form, False, *args)[:2]
