@@ -32,7 +32,7 @@
 //
 // Measured on a B200 (copy rate 6,565 GB/s), 160 M values in 230 tensors: 32-bit step 674 us
 // (28 B per value: 6,650 GB/s), with average 865 us (36 B: 6,650 GB/s): bound by memory.
-// 8-bit step 538 us (16 B: 4,760 GB/s), with average 691 us: bound by its 80 instructions per value (a
+// 8-bit step 549 us (16 B: 4,660 GB/s), with average 693 us: bound by its 80 instructions per value (a
 // fifth of them Philox), issue slots 63% taken.  Gradient norm 108 us (4 B: 5,900 GB/s).  Decoding 160 us (6 B:
 // 6,000 GB/s).  30,000 values in 42 tensors: 8 us (6 us with 8 bits), launch and latency.
 #include "ictc_cuda.h"

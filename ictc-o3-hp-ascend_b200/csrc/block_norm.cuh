@@ -38,10 +38,10 @@
 //   second 1,265 us (5,250);  8,192 rows of C128/lmax 3: 53 us (5,360), 84 us (5,200), 176 us (4,100);
 //   100,000 rows of C128/lmax 0: 76 us (3,380), 104 us (3,920), 221 us (3,010).
 // The forward and the first gradients are near the memory's rate.  The second derivatives at lmax 3 stage 53 KB per
-// row of C128, so two rows are worked on and two are under way per multiprocessor: their eight warps wait on one
-// another's sums and on arrivals (issue slots 37% taken).  Two sets of warps per row, one for degree 3
-// and one for the rest, measured the same (177 us) and were dropped.  At lmax 0 a row is short and the fixed
-// work per tile (sums, barriers, copies) shows.
+// row of C128, so two rows are worked on and two are under way per multiprocessor: eight warps, bound by the
+// latency of their instructions (issue slots 37% taken; with no row written and half of the inputs 600 of 646 us
+// at 32,768 rows).  Two sets of warps per row, one for degree 3 and one for the rest, gave 615 us there but lost at
+// C64 and were dropped.  At lmax 0 a row is short and the fixed work per tile (sums, barriers, copies) shows.
 #pragma once
 
 #include "ictc_common.cuh"
