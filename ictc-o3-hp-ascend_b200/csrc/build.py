@@ -3,7 +3,8 @@
 Each .cu file is compiled to an object in parallel, then linked into
 ``ictc_o3/backends/cuda/libictc_cuda.so`` beside the Python package that
 loads it.  The CUDA runtime is linked statically, so the library carries no
-dependency on a particular libcudart soname.
+dependency on a particular libcudart soname.  host_tensors.cpp becomes a Python
+extension module beside it (g++, against the installed torch and this interpreter).
 
     python build.py [--force] [--verbose]
 """
@@ -12,6 +13,7 @@ import concurrent.futures
 import os
 import subprocess
 import sys
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 PKG = os.path.dirname(HERE)
@@ -19,6 +21,8 @@ REPO = os.path.dirname(PKG)
 INCLUDE = os.path.join(REPO, "include")
 OBJDIR = os.path.join(PKG, "_build")
 OUTPUT = os.path.join(PKG, "ictc_o3", "backends", "cuda", "libictc_cuda.so")
+HOST_SOURCE = os.path.join(HERE, "host_tensors.cpp")
+HOST_OUTPUT = os.path.join(PKG, "ictc_o3", "backends", "cuda", "_host_tensors" + sysconfig.get_config_var("EXT_SUFFIX"))
 NVCC = os.environ.get("NVCC", "nvcc")
 FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
          "-Xcompiler", "-fPIC", "-I" + INCLUDE, "-I" + HERE]
@@ -52,8 +56,29 @@ def _compile(src, force, verbose):
     return obj
 
 
+def build_host(force=False):
+    """The extension module of host_tensors.cpp."""
+    import torch
+    root = os.path.dirname(os.path.abspath(torch.__file__))
+    stamp = max(os.path.getmtime(HOST_SOURCE), os.path.getmtime(os.path.join(root, "version.py")))
+    if not force and os.path.exists(HOST_OUTPUT) and os.path.getmtime(HOST_OUTPUT) >= stamp:
+        return HOST_OUTPUT
+    tmp = HOST_OUTPUT + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+           "-I" + sysconfig.get_paths()["include"], HOST_SOURCE, "-L" + os.path.join(root, "lib"),
+           "-lc10", "-ltorch_cpu", "-ltorch_python", "-o", tmp]
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"g++ failed for host_tensors.cpp:\n{proc.stderr}")
+    os.replace(tmp, HOST_OUTPUT)
+    return HOST_OUTPUT
+
+
 def build(force=False, verbose=False):
     os.makedirs(OBJDIR, exist_ok=True)
+    build_host(force)
     srcs = sources()
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(srcs), os.cpu_count() or 1))) as pool:
         objs = list(pool.map(lambda s: _compile(s, force, verbose), srcs))

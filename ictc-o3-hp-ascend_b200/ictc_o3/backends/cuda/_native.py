@@ -128,6 +128,16 @@ def stream_of(tensor):
     return ctypes.c_void_p(torch.cuda.current_stream(tensor.device).cuda_stream)
 
 
+def host_tensors():
+    """The extension module that reads many tensors' addresses at once (csrc/host_tensors.cpp)."""
+    try:
+        from . import _host_tensors
+    except ImportError as error:
+        raise NativeError(f"_host_tensors is missing or was built for another torch ({error}); "
+                          "run __graft_entry__.build()") from error
+    return _host_tensors
+
+
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 

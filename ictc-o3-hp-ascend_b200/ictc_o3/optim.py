@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import math
 from array import array
-from operator import attrgetter
 
 import torch
 
@@ -25,17 +24,6 @@ def _number(value, name, low, high=math.inf, open_low=False):
     if not (low < value if open_low else low <= value) or not value < high:
         raise ValueError(f"{name} is outside its range")
     return value
-
-
-# what a step needs to know of all its tensors: (FP32?, device, values, contiguous?), column by column
-_gradient, _dtype = attrgetter("grad"), attrgetter("dtype")
-_device, _numel = torch.Tensor.get_device, torch.Tensor.numel
-_contiguous, _address = torch.Tensor.is_contiguous, torch.Tensor.data_ptr
-
-
-def _columns(tensors):
-    return (list(map(_dtype, tensors)), list(map(_device, tensors)), list(map(_numel, tensors)),
-            list(map(_contiguous, tensors)))
 
 
 def _hyperparameters(group):
@@ -96,6 +84,7 @@ class AdamW(torch.optim.Optimizer):
         super().add_param_group(param_group)
 
     def _build(self):
+        from ictc_o3.backends.cuda._native import host_tensors
         from ictc_o3.backends.cuda.adamw import BLOCK, TensorTable, blocks_of
         for group in self.param_groups:
             _hyperparameters(group)
@@ -134,9 +123,9 @@ class AdamW(torch.optim.Optimizer):
         self._params, self._flat, self._device = params, flat, device
         self._places = [None if flat[k] is None else flat[k].data_ptr()
                         for k in ("m", "v", "m_scale", "v_scale", "average", "steps", "rates")]
-        self._expected = ([torch.float32] * len(params), [device.index] * len(params), [p.numel() for p in params],
-                          [True] * len(params))
-        self._full = all(p.numel() for p in params)
+        self._sizes = array("q", [p.numel() for p in params])
+        self._weights, self._grads = array("Q", [0] * len(params)), array("Q", [0] * len(params))
+        self._host = host_tensors()
         self._table = table
         self._empty = table.workspace.data_ptr()      # stands for the gradient of a tensor without values
 
@@ -146,31 +135,28 @@ class AdamW(torch.optim.Optimizer):
     # -- one step -----------------------------------------------------------
 
     def _gather(self):
-        """Addresses of weights and gradients (0: no gradient), the updated weights, and
+        """Fill the arrays of addresses (0: no gradient); returns how many have a gradient, and
         temporaries that must outlive the launch."""
-        params, expected = self._params, self._expected
-        grads = list(map(_gradient, params))
-        live, kept = params, ()
-        try:      # as a rule: a dense, contiguous gradient everywhere
-            fine = _columns(grads) == expected
-            places = list(map(_address, grads)) if fine else None
-        except (AttributeError, TypeError, RuntimeError):      # None, or a layout without an address
-            fine = False
-        if not fine:
-            there = [g is not None for g in grads]
-            live = [p for p, t in zip(params, there) if t]
-            expected = tuple([e for e, t in zip(column, there) if t] for column in expected)
-        if _columns(live) != expected:
-            raise ValueError("a parameter has changed its type, device, size or layout since the optimizer was built")
-        if not fine:
-            given = [g for g in grads if g is not None]
-            if any(g.layout is not torch.strided for g in given) or _columns(given)[:3] != expected[:3]:
+        weights, grads = self._weights, self._grads
+        live = self._host.gather(self._params, self._sizes.buffer_info()[0], self._device.index,
+                                 weights.buffer_info()[0], grads.buffer_info()[0], self._empty)
+        if live >= 0:
+            return live, None
+        # some tensor is not what it was, or a gradient is not contiguous
+        kept = [None if p.grad is None else p.grad.detach() for p in self._params]
+        for i, (p, g, size) in enumerate(zip(self._params, kept, self._sizes)):
+            if g is None:
+                continue
+            if p.dtype is not torch.float32 or p.device != self._device or p.numel() != size or not p.is_contiguous():
+                raise ValueError("a parameter has changed its type, device, size or layout since the optimizer was built")
+            if (g.layout is not torch.strided or g.dtype is not torch.float32 or g.device != self._device
+                    or g.numel() != size):
                 raise ValueError("gradients must be dense CUDA FP32 tensors of their parameter's size")
-            kept = [None if g is None else g.detach().contiguous() for g in grads]
-            places = [0 if g is None else g.data_ptr() for g in kept]
-        if not self._full:      # a tensor without values has no address, but its steps count
-            places = [self._empty if g is not None and not g.numel() else k for g, k in zip(grads, places)]
-        return array("Q", list(map(_address, params))), array("Q", places), live, kept
+            kept[i] = g.contiguous().resolve_neg()
+        for i, (p, g) in enumerate(zip(self._params, kept)):
+            weights[i] = 0 if g is None else p.data_ptr()
+            grads[i] = 0 if g is None else g.data_ptr() if g.numel() else self._empty
+        return sum(g is not None for g in kept), kept
 
     def step(self, closure=None):
         loss = None
@@ -178,10 +164,10 @@ class AdamW(torch.optim.Optimizer):
             with torch.enable_grad():
                 loss = closure()
         groups = [_hyperparameters(group) for group in self.param_groups]
-        weights, grads, live, kept = self._gather()
+        live, kept = self._gather()
         if not live:
             return loss
-        w, g = weights.buffer_info()[0], grads.buffer_info()[0]
+        w, g = self._weights.buffer_info()[0], self._grads.buffer_info()[0]
         use_norm = self.max_norm is not None or self.skip_nonfinite
         if use_norm:
             self._table.grad_norm(g, self.max_norm, self.skip_nonfinite)
@@ -193,7 +179,7 @@ class AdamW(torch.optim.Optimizer):
                              use_norm=use_norm)
             first += count
         del kept                     # copies of gradients: their memory is reused on this stream only
-        torch.autograd.graph.increment_version(live)
+        self._host.changed(self._params, g)
         return loss
 
     def mark_updated(self):

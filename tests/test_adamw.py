@@ -98,3 +98,24 @@ def test_native_entry_points_validate_before_launching():
     assert lib.ictc_adamw_decode(some, some, some, some, 255, some, some, None) == -1
     assert lib.ictc_adamw_decode(None, None, None, None, 256, None, None, None) == -1
     assert lib.ictc_adamw_decode(None, None, None, None, 0, None, None, None) == 0
+
+
+def test_host_addresses():
+    """The extension module refuses what is not a list of tensors and finds CPU tensors unfit (no GPU needed)."""
+    from array import array
+    from ictc_o3.backends.cuda._native import host_tensors
+    host = host_tensors()
+    params = [torch.nn.Parameter(torch.zeros(n)) for n in (3, 5)]
+    sizes, weights, grads = array("q", [3, 5]), array("Q", [9, 9]), array("Q", [9, 9])
+    args = (sizes.buffer_info()[0], 0, weights.buffer_info()[0], grads.buffer_info()[0], 1)
+    assert host.gather(params, *args) == 0 and list(weights) == list(grads) == [0, 0]
+    params[1].grad = torch.zeros(5)
+    assert host.gather(params, *args) == -2                 # the second is not on the device
+    version = [p._version for p in params]
+    present = array("Q", [0, 7])
+    host.changed(params, present.buffer_info()[0])
+    assert [p._version - v for p, v in zip(params, version)] == [0, 1]
+    for bad in (lambda: host.gather(tuple(params), *args), lambda: host.gather([1], *args),
+                lambda: host.gather(params, *args[:3]), lambda: host.changed(params), lambda: host.gather(params, "x", *args[1:])):
+        with pytest.raises(TypeError):
+            bad()

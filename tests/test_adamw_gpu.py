@@ -277,6 +277,18 @@ def test_other_stream_and_strided_gradient(cuda_device):
     assert torch.equal(a, b)
 
 
+def test_negated_view_as_gradient(cuda_device):
+    """An imaginary part of a lazily conjugated tensor stores the values with the other sign."""
+    from ictc_o3.optim import AdamW
+    a, b = (torch.nn.Parameter(torch.zeros(1, device=cuda_device)) for _ in range(2))
+    a.grad = torch.full((1,), 1 + 2j, device=cuda_device).conj().imag
+    assert a.grad.is_neg() and a.grad.is_contiguous()
+    b.grad = a.grad.resolve_neg()
+    for p in (a, b):
+        AdamW([p], **HYPER).step()
+    assert float(a) == float(b) > 0
+
+
 def test_tiny_gradients_and_epsilon(cuda_device):
     """Second moments below FP32's normal range still divide (no flush to zero), in both forms."""
     from ictc_o3.optim import AdamW
