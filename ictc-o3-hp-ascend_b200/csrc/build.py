@@ -57,8 +57,11 @@ def _compile(src, force, verbose):
 
 
 def build_host(force=False):
-    """The extension module of host_tensors.cpp."""
-    import torch
+    """The extension module of host_tensors.cpp; without torch it has no user and is left out."""
+    try:
+        import torch
+    except ImportError:
+        return None
     root = os.path.dirname(os.path.abspath(torch.__file__))
     stamp = max(os.path.getmtime(HOST_SOURCE), os.path.getmtime(os.path.join(root, "version.py")))
     if not force and os.path.exists(HOST_OUTPUT) and os.path.getmtime(HOST_OUTPUT) >= stamp:
