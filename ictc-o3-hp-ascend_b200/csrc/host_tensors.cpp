@@ -1,5 +1,5 @@
-// Addresses of many tensors in one call: the only part of this package that reads torch's
-// own structures.  An optimizer step needs the addresses of all weights and gradients and
+// The only part of this package that reads torch's own structures: addresses of many tensors in one
+// call, and the stream on which a leaf's gradient is added up.  An optimizer step needs the addresses of all weights and gradients and
 // must see that each is still a dense, contiguous FP32 tensor of its size on its device: eleven Python
 // attribute reads per tensor, 0.55 us, against 0.03 us here (42 tensors: a step's host time 45 -> 21 us).
 // The kernels keep their plain C interface.
@@ -7,7 +7,9 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/autograd/variable.h>
 
 namespace {
 
@@ -84,11 +86,30 @@ PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// accumulates_on_default_stream(leaf): whether the leaf's gradient is added up on the device's default
+// stream, as it is while a graph recorded there lives.
+PyObject* accumulates_on_default_stream(PyObject*, PyObject* leaf) {
+  if (!THPVariable_Check(leaf)) {
+    PyErr_SetString(PyExc_TypeError, "accumulates_on_default_stream takes a tensor");
+    return nullptr;
+  }
+  try {
+    const auto node = torch::autograd::impl::try_get_grad_accumulator(THPVariable_Unpack(leaf));
+    const auto stream = node ? node->stream() : std::nullopt;
+    return PyBool_FromLong(stream.has_value() && stream->id() == 0);
+  } catch (const std::exception& e) {
+    PyErr_SetString(PyExc_RuntimeError, e.what());
+    return nullptr;
+  }
+}
+
 PyMethodDef methods[] = {
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(gather)), METH_FASTCALL,
      "Addresses of tensors and their gradients."},
     {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(changed)), METH_FASTCALL,
      "Raise the tensors' version counters."},
+    {"accumulates_on_default_stream", accumulates_on_default_stream, METH_O,
+     "Whether a leaf's gradient is added up on the default stream."},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_tensors", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

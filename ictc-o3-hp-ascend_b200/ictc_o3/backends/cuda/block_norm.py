@@ -151,6 +151,18 @@ def _runs(node):
         return True
 
 
+def _check_capture(ctx):
+    """A captured backward pass hands each leaf's gradient to the stream of the oldest living graph with this
+    leaf.  If that is the default stream, which cannot take part in a capture, the process would end: refused here."""
+    if not torch.cuda.is_current_stream_capturing():
+        return
+    for node, _ in ctx.next_functions:
+        leaf = getattr(node, "variable", None)
+        if leaf is not None and _native.host_tensors().accumulates_on_default_stream(leaf):
+            raise RuntimeError("a backward pass cannot be captured while a graph of the same leaves, recorded on the "
+                               "default stream, lives: drop its outputs first")
+
+
 class _Block(torch.autograd.Function):
     @staticmethod
     def forward(ctx, form, stream, branch, gate, post, scale, pre):
@@ -163,6 +175,7 @@ class _Block(torch.autograd.Function):
     @staticmethod
     def backward(ctx, *cotangents):
         form = ctx.form
+        _check_capture(ctx)
         stream, branch, gate, post, scale, pre = ctx.saved_tensors
         p = cotangents[0] if branch is not None else None
         q = cotangents[-1] if form.norm else None
@@ -197,6 +210,7 @@ class _BlockGrad(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dot_stream, dot_branch, dot_gate, *dot_weights):
         form = ctx.form
+        _check_capture(ctx)
         saved = ctx.saved_tensors
         stream, branch, gate, post, scale, pre, p, q = saved
         need = ctx.needs_input_grad[3:]

@@ -44,7 +44,10 @@ def force_loss(result, batch, energy_target, force_target, *, energy_weight=1.0,
 def train_step(model, optimizer, positions, atomic_numbers, batch, edge_src, edge_dst, edge_shifts, cell, energy_target,
                force_target, *, energy_weight=1.0, force_weight=100.0):
     """One step on a prebuilt batch of graphs (arguments of ``energy_and_forces``): the loss before
-    it, as a device scalar that was not waited for."""
+    it, as a device scalar that was not waited for.  Not to be captured: what the model derives from its weights
+    (packed radial weights, folded tables) is renewed by the host, so replays would use old ones."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("a training step cannot be captured into a CUDA graph")
     optimizer.zero_grad(set_to_none=True)
     result = energy_and_forces(model, positions, atomic_numbers, batch, edge_src, edge_dst, edge_shifts, cell,
                                training=True)

@@ -119,3 +119,12 @@ def test_host_addresses():
                 lambda: host.gather(params, *args[:3]), lambda: host.changed(params), lambda: host.gather(params, "x", *args[1:])):
         with pytest.raises(TypeError):
             bad()
+
+
+def test_where_gradients_are_added_up():
+    from ictc_o3.backends.cuda._native import host_tensors
+    leaf = torch.zeros(2, requires_grad=True)
+    for graph in (None, leaf * 2):      # on the CPU there is no stream
+        assert host_tensors().accumulates_on_default_stream(leaf) is False
+    with pytest.raises(TypeError):
+        host_tensors().accumulates_on_default_stream(None)

@@ -10,6 +10,7 @@ T: r^3 h' <h', b q>: 3 x 38 rho + 38 + 38 + 48 + 6 < 250 rho.  dbranch, dgate: 2
 400 rho.  Second derivatives take T, tau (400 rho + 28 + 10) or both times r^5 (5 x 38 rho)
 and two sums (96): below 400 + 440 + 190 + 96 + 20 < 1200 rho.  A sum over N rows adds N.
 """
+import gc
 import itertools
 
 import pytest
@@ -454,6 +455,36 @@ def test_first_call_inside_a_capture(cuda_device, monkeypatch):
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(held, step()))
     assert block_norm_status() == 0
+
+
+def test_backward_inside_a_capture(cuda_device):
+    """A captured backward pass gives the eager gradients, and is refused while a graph of the same leaves lives."""
+    from ictc_o3.ops.block_norm import residual_block_norm
+    t = inputs(50, 20, 1)
+    leaves = [t[k].detach().requires_grad_() for k in ("stream", "branch", "scale")]
+
+    def step():
+        out = residual_block_norm(leaves[0], leaves[1], scale=leaves[2], norm=True, channels=20, lmax=1)
+        return out, lambda: torch.autograd.backward(out, [t["p"], t["q"]])
+
+    out, backward = step()
+    backward()
+    want = [x.grad.clone() for x in leaves]
+    for x in leaves:
+        x.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        with torch.cuda.graph(graph):
+            step()[1]()
+    del out, backward, graph
+    gc.collect()
+    for x in leaves:
+        x.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()[1]()
+    graph.replay()
+    assert all(torch.equal(x.grad, w) for x, w in zip(leaves, want))
 
 
 def test_refusals(cuda_device):

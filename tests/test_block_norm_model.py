@@ -117,3 +117,10 @@ def test_slab_decomposition_with_block_norms(tmp_path):
         torch.testing.assert_close(out["energy"], energy, rtol=1e-9, atol=1e-9)
         torch.testing.assert_close(out["virial"], virial, rtol=1e-8, atol=1e-8)
     torch.testing.assert_close(joined, forces, rtol=1e-8, atol=1e-8)
+
+
+def test_training_step_refuses_a_capture(monkeypatch):
+    from mace_ictc.training import train_step
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(RuntimeError, match="cannot be captured"):
+        train_step(*[None] * 11)
