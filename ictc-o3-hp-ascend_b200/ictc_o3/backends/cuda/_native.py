@@ -141,15 +141,22 @@ def host_tensors():
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
+def _address(tensor, name):
+    # a host tensor in the place of a number (a size under torch.jit.trace) would pass its address as that number
+    if not tensor.is_cuda:
+        raise TypeError(f"{name} takes addresses of CUDA tensors only")
+    return tensor.data_ptr()
+
+
 def launch(device, name, *args):
-    """``call`` with ``device`` current and its current stream as the last argument; tensors may be
+    """``call`` with ``device`` current and its current stream as the last argument; CUDA tensors may be
     given for their addresses (None: NULL)."""
+    args = [_address(a, name) if isinstance(a, torch.Tensor) else a for a in args]
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return launch(device, name, *args)
     stream = torch.cuda.current_stream(device).cuda_stream if _raw_stream is None else _raw_stream(device.index)
-    status = getattr(_lib or library(), name)(
-        *[a.data_ptr() if isinstance(a, torch.Tensor) else a for a in args], stream)
+    status = getattr(_lib or library(), name)(*args, stream)
     if status != 0:
         check(status, name)
 

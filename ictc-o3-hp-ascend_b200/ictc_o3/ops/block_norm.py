@@ -11,8 +11,8 @@ start of the next are
 with weights and gates per degree and channel.  r depends on a degree's length only, so the
 operator commutes with rotations.  For lmax = 0 a row is a plain vector of C channels.
 Forward, first and second derivatives are one kernel each (forces and force-loss training
-need both); higher ones go through torch operations.  All of it can be captured into a CUDA graph;
-a backward pass is refused there while a graph of the same leaves recorded on the default stream lives.
+need both); higher ones go through torch operations.  ``torch.jit.trace`` is refused.  All of it can be
+captured into a CUDA graph; a backward pass is refused there while a graph of the same leaves recorded on the default stream lives.
 """
 from __future__ import annotations
 
@@ -44,6 +44,8 @@ def _form(channels, lmax, layout, eps, norm):
 
 
 def _check(form, rows, weights, gate=None):
+    if torch.jit.is_tracing():      # sizes are tensors there, and a trace would hold the outputs' allocation alone
+        raise ValueError("block norms cannot be traced; the CUDA backend requires ordinary eager autograd")
     c, degrees = form.channels, form.lmax + 1
     n = rows[0].shape[0] if rows[0].ndim else 0
     tensors = [*rows, *weights] if gate is None else [*rows, *weights, gate]
