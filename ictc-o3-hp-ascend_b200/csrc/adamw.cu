@@ -5,7 +5,7 @@
 //   w = w (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
 //   average = d average + (1 - d) w                                   (optional)
 // clip = min(1, max_norm / (|g| + 1e-6)) comes from a first pass over the gradients
-// (grad_norm_kernel) when clipping or skipping of non-finite steps is asked for.
+// (grad_norm_kernel) when clipping or skipping of non-finite steps is asked for; it is NaN where |g| is.
 //
 // Work is cut into chunks of consecutive values of one tensor; a static device table gives
 // each chunk's tensor, place and count, and the addresses of weights and gradients travel
@@ -270,7 +270,8 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const __grid_consta
     if (last_launch) {
       const float norm = (float)sqrt(sum);
       a.ws->norm = norm;
-      a.ws->clip = clip ? fminf(__fmul_rn(__frcp_rn(__fadd_rn(norm, 1e-6f)), max_norm), 1.f) : 1.f;
+      const float share = __fmul_rn(__frcp_rn(__fadd_rn(norm, 1e-6f)), max_norm);
+      a.ws->clip = clip && !(share > 1.f) ? share : 1.f;      // a NaN norm stays one, as a minimum would not
       a.ws->skip = skip_bad && !isfinite(sum);
     }
     a.ws->norm_ticket = 0;

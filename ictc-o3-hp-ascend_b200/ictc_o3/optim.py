@@ -48,7 +48,8 @@ class AdamW(torch.optim.Optimizer):
     power-of-two scale per 256 values (the last block of a tensor may be shorter), rounded
     stochastically from ``seed``, the tensor's step and the value's place, so that
     equal inputs give equal results.  A block whose new moments are not finite is left as it was.
-    ``max_norm``: gradients are scaled by min(1, max_norm / (|g| + 1e-6)), |g| over all of them.
+    ``max_norm``: gradients are scaled by min(1, max_norm / (|g| + 1e-6)), |g| over all of them; a NaN among
+    them makes that factor NaN (moments in 8 bits, and their weights, then stay as they were).
     ``skip_nonfinite``: a step with an infinite or NaN gradient changes nothing and is not counted.
     ``ema_decay``: keeps average = d average + (1 - d) weight in ``state[p]["ema"]``.
 

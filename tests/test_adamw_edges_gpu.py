@@ -1,0 +1,52 @@
+"""AdamW where a step or a state dict is out of the ordinary."""
+import pytest
+import torch
+
+from oracle import adamw_oracle
+from test_adamw_gpu import HYPER, make, within
+
+pytestmark = pytest.mark.gpu
+
+
+def snapshot(opt, params):
+    return [x.detach().clone() for p in params for k, x in (("", p), *opt.state[p].items()) if k != "step"]
+
+
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_clipping_with_a_nonfinite_norm(bits, bad, cuda_device):
+    """The factor min(1, max_norm / (|g| + 1e-6)) of a NaN norm is NaN and that of an infinite one 0: a NaN
+    spoils the whole step (8-bit blocks then stay as they were), an infinity its own value, and the rest takes a
+    step with zero gradients."""
+    from ictc_o3.optim import AdamW
+    sizes = [4000, 700, 3]
+    params, twins = make(sizes, cuda_device, seed=21), make(sizes, cuda_device, seed=21)
+    opts = [AdamW(x, **HYPER, state_bits=bits, max_norm=1.0, ema_decay=0.5, seed=4) for x in (params, twins)]
+    for opt in opts:
+        opt.step()
+    params[0].grad[1234] = bad
+    for q in twins:
+        q.grad.zero_()
+    kept = snapshot(opts[0], params)
+    for opt in opts:
+        opt.step()
+    assert not torch.isfinite(opts[0].grad_norm)
+    assert all(int(opts[0].state[p]["step"]) == 2 for p in params)
+    if bad != bad:
+        if bits == 32:
+            assert all(bool(x.isnan().all()) for x in snapshot(opts[0], params))
+        else:
+            assert all(torch.equal(a, b) for a, b in zip(kept, snapshot(opts[0], params)))
+        return
+    spoilt = torch.zeros(4000, dtype=torch.bool, device=cuda_device)
+    if bits == 32:
+        spoilt[1234] = True
+        assert torch.isnan(params[0][1234]) and torch.isnan(opts[0].state[params[0]]["ema"][1234])
+    else:
+        spoilt[1234 // 256 * 256:1234 // 256 * 256 + 256] = True
+        assert torch.equal(params[0][spoilt], kept[0][spoilt])
+    for p, q in zip(params, twins):
+        good = ~spoilt if p is params[0] else slice(None)
+        assert torch.equal(p[good], q[good])
+        for key in ("exp_avg", "exp_avg_sq", "ema"):
+            assert torch.equal(opts[0].state[p][key][good], opts[1].state[q][key][good])
