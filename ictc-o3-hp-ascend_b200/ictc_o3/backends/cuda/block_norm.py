@@ -109,8 +109,11 @@ def status_word(device):
     return word
 
 
-def _dense(x):
-    return None if x is None else x.contiguous()
+def dense(x):
+    """``x`` with its values one after another at its address: contiguous, and no lazily negated view."""
+    if x is None or (x.is_contiguous() and not x.is_neg()):
+        return x
+    return x.resolve_neg().contiguous()
 
 
 def _forward(form, keep, stream, branch, gate, post, scale, pre):
@@ -191,7 +194,7 @@ class _Block(torch.autograd.Function):
         need_branch = need_branch and _runs(at_branch)
         runs = any(n and _runs(node) for n, node in zip(need_weights, at_weights))
         need = (need_stream, need_branch, need_gate, *[n and runs for n in need_weights])
-        args = (form, ctx.rates, need, stream, branch, gate, post, scale, pre, _dense(p), _dense(q))
+        args = (form, ctx.rates, need, stream, branch, gate, post, scale, pre, dense(p), dense(q))
         grads = _BlockGrad.apply(*args) if torch.is_grad_enabled() else _first(*args)
         dx = p if q is None else grads[0]
         return (None, dx if need[0] else None, *grads[1:])
@@ -238,13 +241,13 @@ class _BlockGrad(torch.autograd.Function):
             out[0] = out[5] = out[7] = None
         partial = _partial(form, stream, any(t is not None for t in out[3:6]))
         launch(stream.device, "ictc_block_second", stream, branch, gate, post, scale, pre, *ctx.rates, p, q,
-               *[_dense(d) for d in dots[:3]], stream.shape[0], form.channels, form.lmax, LAYOUTS[form.layout], *out,
+               *[dense(d) for d in dots[:3]], stream.shape[0], form.channels, form.lmax, LAYOUTS[form.layout], *out,
                partial, status_word(stream.device))
         return (None, None, None, *out)
 
 
 def block(form, stream, branch, gate, post, scale, pre):
-    """(stream', normed) of contiguous arguments; without anything to differentiate no graph is made."""
+    """(stream', normed) of arguments that went through ``dense``; without anything to differentiate no graph is made."""
     args = (stream, branch, gate, post, scale, pre)
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args]):
         out = _Block.apply(form, *args)

@@ -21,7 +21,7 @@ import functools
 import torch
 
 from ictc_o3.backends.cuda import _native
-from ictc_o3.backends.cuda.block_norm import LAYOUTS, Form, block, status_word
+from ictc_o3.backends.cuda.block_norm import LAYOUTS, Form, block, dense, status_word
 from ictc_o3.backends.cuda.runtime import require_cuda_fp32
 
 __all__ = ["degree_norm", "residual_block_norm", "DegreeNorm", "ResidualBlockNorm",
@@ -62,10 +62,6 @@ def _check(form, rows, weights, gate=None):
         raise ValueError("Gates must have shape [N,(L+1)*C] or [N,L+1,C]")
 
 
-def _contiguous(x):
-    return x if x is None or x.is_contiguous() else x.contiguous()
-
-
 def block_norm_status(device="cuda"):
     """0, or what a kernel of this module left after a copy into shared memory did not land within two
     seconds (its results are then not valid).  Reads one int from the device: for tests and after a step."""
@@ -81,7 +77,7 @@ def degree_norm(features, weight=None, *, channels, lmax, layout="mul_ir", eps=1
     """weight * r(features) * features: the norm before the first block."""
     form = _form(channels, lmax, layout, eps, True)
     _check(form, (features,), () if weight is None else (weight,))
-    return block(form, _contiguous(features), None, None, None, None, _contiguous(weight))[1]
+    return block(form, dense(features), None, None, None, None, dense(weight))[1]
 
 
 def residual_block_norm(stream, branch, *, channels, lmax, post_weight=None, scale=None, gate=None, pre_weight=None,
@@ -98,8 +94,8 @@ def residual_block_norm(stream, branch, *, channels, lmax, post_weight=None, sca
     _check(form, (stream, branch), tuple(w for w in (post_weight, scale, pre_weight) if w is not None), gate)
     if gate is not None and gate.ndim == 3:
         gate = gate.reshape(gate.shape[0], (lmax + 1) * channels)
-    return block(form, _contiguous(stream), _contiguous(branch), _contiguous(gate), _contiguous(post_weight),
-                 _contiguous(scale), _contiguous(pre_weight))
+    return block(form, dense(stream), dense(branch), dense(gate), dense(post_weight),
+                 dense(scale), dense(pre_weight))
 
 
 class DegreeNorm(torch.nn.Module):

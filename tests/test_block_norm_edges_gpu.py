@@ -1,0 +1,39 @@
+"""Block norms with tensors and calls out of the ordinary."""
+import pytest
+import torch
+
+from test_block_norm_gpu import inputs
+
+pytestmark = pytest.mark.gpu
+NAMES = ("stream", "branch", "gate", "post_weight", "scale", "pre_weight")
+FORM = {"channels": 12, "lmax": 2}
+
+
+def call(t):
+    from ictc_o3.ops.block_norm import residual_block_norm
+    return residual_block_norm(t["stream"], t["branch"], **{k: t[k] for k in NAMES[2:]}, **FORM)
+
+
+def all_of(t):
+    """Outputs, first gradients and their adjoints."""
+    leaves = [t[k] for k in NAMES]
+    out = call(t)
+    first = torch.autograd.grad(out, leaves, [t["p"], t["q"]], create_graph=True)
+    second = torch.autograd.grad(first[:3], [*leaves, t["p"], t["q"]], [t["d_stream"], t["d_branch"], t["d_gate"]])
+    return [x.detach() for x in (*out, *first, *second)]
+
+
+@pytest.mark.parametrize("name", [*NAMES, "p", "q", "d_stream", "d_branch", "d_gate"])
+def test_negated_views(name, cuda_device):
+    """A lazily negated tensor is contiguous and stores the other sign."""
+    from ictc_o3.ops.block_norm import degree_norm
+    t = inputs(23, 12, 2, seed=3)
+    want = all_of(t)
+    t[name] = torch._neg_view(t[name].detach().neg()).requires_grad_()
+    assert t[name].is_neg() and t[name].is_contiguous()
+    assert all(torch.equal(a, b) for a, b in zip(all_of(t), want))
+    with torch.no_grad():
+        assert all(torch.equal(a, b) for a, b in zip(call(t), want))
+        if name in ("stream", "pre_weight"):
+            plain = degree_norm(t["stream"].resolve_neg(), t["pre_weight"].resolve_neg(), **FORM)
+            assert torch.equal(degree_norm(t["stream"], t["pre_weight"], **FORM), plain)
