@@ -10,6 +10,7 @@ from __future__ import annotations
 from typing import NamedTuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _native
 from ._native import launch
@@ -116,6 +117,15 @@ def dense(x):
     return x.resolve_neg().contiguous()
 
 
+def _refuse_tangents(*tensors):
+    """Forward-mode derivatives have no kernel: outputs written by address would drop their tangents."""
+    if getattr(forward_ad, "_current_level", 0) < 0:      # no dual level is open
+        return
+    if any([t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors]):
+        raise ValueError("block norms have no forward-mode derivatives; the CUDA backend requires ordinary eager "
+                         "autograd")
+
+
 def _forward(form, keep, stream, branch, gate, post, scale, pre):
     """(stream', normed, r1, r2): what is not produced, or without ``keep`` not kept, is None."""
     n, device = stream.shape[0], stream.device
@@ -179,6 +189,7 @@ class _Block(torch.autograd.Function):
     def backward(ctx, *cotangents):
         form = ctx.form
         _check_capture(ctx)
+        _refuse_tangents(*cotangents)
         stream, branch, gate, post, scale, pre = ctx.saved_tensors
         p = cotangents[0] if branch is not None else None
         q = cotangents[-1] if form.norm else None
@@ -218,6 +229,7 @@ class _BlockGrad(torch.autograd.Function):
         stream, branch, gate, post, scale, pre, p, q = saved
         need = ctx.needs_input_grad[3:]
         dots = (dot_stream, dot_branch, dot_gate, *dot_weights)
+        _refuse_tangents(*dots)
         if all(d is None for d in dots):
             return (None,) * 11
         if torch.is_grad_enabled() or any(d is not None for d in dot_weights):
@@ -249,6 +261,7 @@ class _BlockGrad(torch.autograd.Function):
 def block(form, stream, branch, gate, post, scale, pre):
     """(stream', normed) of arguments that went through ``dense``; without anything to differentiate no graph is made."""
     args = (stream, branch, gate, post, scale, pre)
+    _refuse_tangents(*args)
     if torch.is_grad_enabled() and any([t is not None and t.requires_grad for t in args]):
         out = _Block.apply(form, *args)
         return (None, out[0]) if branch is None else out if form.norm else (out[0], None)

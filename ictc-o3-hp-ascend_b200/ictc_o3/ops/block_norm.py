@@ -11,7 +11,8 @@ start of the next are
 with weights and gates per degree and channel.  r depends on a degree's length only, so the
 operator commutes with rotations.  For lmax = 0 a row is a plain vector of C channels.
 Forward, first and second derivatives are one kernel each (forces and force-loss training
-need both); higher ones go through torch operations.  ``torch.jit.trace`` is refused.  All of it can be
+need both); higher ones go through torch operations.  ``torch.jit.trace`` and forward-mode
+derivatives are refused.  All of it can be
 captured into a CUDA graph; a backward pass is refused there while a graph of the same leaves recorded on the default stream lives.
 """
 from __future__ import annotations

@@ -37,3 +37,33 @@ def test_negated_views(name, cuda_device):
         if name in ("stream", "pre_weight"):
             plain = degree_norm(t["stream"].resolve_neg(), t["pre_weight"].resolve_neg(), **FORM)
             assert torch.equal(degree_norm(t["stream"], t["pre_weight"], **FORM), plain)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_forward_mode_is_refused(name, cuda_device):
+    """No kernel computes tangents, with or without a graph; other tensors may be dual meanwhile."""
+    from torch.autograd import forward_ad
+    t = inputs(7, 12, 2)
+    want = [x.detach() for x in call(t)]
+    for grad in (False, True):
+        u = {k: v.detach().requires_grad_(grad) for k, v in t.items()}
+        with forward_ad.dual_level():
+            assert all(torch.equal(a, b) for a, b in zip(call(u), want))
+            u[name] = forward_ad.make_dual(u[name], torch.ones_like(u[name]))
+            with pytest.raises(ValueError, match="forward-mode"):
+                call(u)
+
+
+@pytest.mark.parametrize("second", [False, True])
+def test_forward_mode_over_a_backward_pass_is_refused(second, cuda_device):
+    from torch.autograd import forward_ad
+    t = inputs(7, 12, 2)
+    out = call(t)
+    cotangents = [t["p"], t["q"]]
+    if second:
+        out = torch.autograd.grad(out, [t["branch"]], cotangents, create_graph=True)
+        cotangents = [t["d_branch"]]
+    with forward_ad.dual_level():
+        cotangents[0] = forward_ad.make_dual(cotangents[0].detach(), torch.ones_like(cotangents[0]))
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(out, [t["branch"], t["scale"]], cotangents)
