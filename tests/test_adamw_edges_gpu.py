@@ -50,3 +50,31 @@ def test_clipping_with_a_nonfinite_norm(bits, bad, cuda_device):
         assert torch.equal(p[good], q[good])
         for key in ("exp_avg", "exp_avg_sq", "ema"):
             assert torch.equal(opts[0].state[p][key][good], opts[1].state[q][key][good])
+
+
+@pytest.mark.parametrize("decay", [0.0, 0.3, 0.5, 0.9, 0.999, 0.9999, 0.99999])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_weight_average(bits, decay, cuda_device):
+    """d average + (1 - d) weight: two half steps for the rounded factor times the distance, one for the
+    difference and one for the sum, and an average equal to its weights stays there."""
+    from ictc_o3.optim import AdamW
+    params = make([3000, 5], cuda_device, seed=31)
+    opt = AdamW(params, **HYPER, state_bits=bits, ema_decay=decay)
+    saved = opt.state_dict()
+    old = [p.detach() * 1.5 - 0.25 for p in params]
+    for i, e in enumerate(old):
+        saved["state"][i] = {**saved["state"][i], "ema": e}
+    opt.load_state_dict(saved)
+    opt.step()
+    share = min(decay, 1 - decay)
+    for p, e in zip(params, old):
+        w, e = p.detach().double(), e.double()
+        want = decay * e + (1 - decay) * w
+        within(opt.state[p]["ema"], want, 1.01 * adamw_oracle.U * (2 * share * (w - e).abs() + want.abs()), "average")
+    still = make([700, 5], cuda_device, seed=32)
+    opt = AdamW(still, lr=0.0, weight_decay=0.0, state_bits=bits, ema_decay=decay)
+    start = [p.detach().clone() for p in still]
+    for _ in range(300):
+        opt.step()
+    for p, w in zip(still, start):
+        assert torch.equal(p, w) and torch.equal(opt.state[p]["ema"], w)
