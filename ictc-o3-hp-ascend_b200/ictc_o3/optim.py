@@ -265,7 +265,7 @@ class AdamW(torch.optim.Optimizer):
                 else:
                     value.fill_(1 if key.endswith("exponent") else 0)
         self._flat["steps"].copy_(torch.tensor(steps, dtype=torch.int64))
-        if all(v.device == self._device for v in values):
+        if values and all(v.device == self._device for v in values):
             torch._foreach_copy_(to, values)
         else:
             for mine, value in zip(to, values):

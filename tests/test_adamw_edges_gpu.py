@@ -78,3 +78,33 @@ def test_weight_average(bits, decay, cuda_device):
         opt.step()
     for p, w in zip(still, start):
         assert torch.equal(p, w) and torch.equal(opt.state[p]["ema"], w)
+
+
+@pytest.mark.parametrize("ema", [None, 0.9])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dicts_with_missing_entries(bits, ema, cuda_device):
+    """Parameters without an entry start anew, all of them or some."""
+    from ictc_o3.optim import AdamW
+    params = make([700, 0, 300], cuda_device, seed=41)
+    opt = AdamW(params, **HYPER, state_bits=bits, ema_decay=ema)
+    for kept in ((), (0,), (1,), (0, 2)):
+        opt.step()
+        opt.step()
+        saved = opt.state_dict()
+        saved = {"state": {i: {k: v.clone() for k, v in saved["state"][i].items()} for i in kept},
+                 "param_groups": saved["param_groups"]}
+        opt.load_state_dict(saved)
+        for i, p in enumerate(params):
+            state = opt.state[p]
+            if i in kept:
+                assert int(state["step"]) == 2
+                assert all(torch.equal(state[k], v) for k, v in saved["state"][i].items())
+            else:
+                assert int(state["step"]) == 0 and not state["exp_avg"].any() and not state["exp_avg_sq"].any()
+                assert ema is None or torch.equal(state["ema"], p.detach())
+                assert bits == 32 or bool((state["exp_avg_exponent"] == 1).all())
+        for p in params:
+            opt.state[p]["step"].zero_()
+    if bits == 32:      # the library's, before its first step
+        opt.load_state_dict(torch.optim.AdamW(make([700, 0, 300], cuda_device), lr=0.125).state_dict())
+        assert opt.param_groups[0]["lr"] == 0.125 and not opt.state[params[0]]["exp_avg"].any()
