@@ -210,10 +210,20 @@ class AdamW(torch.optim.Optimizer):
 
     # -- checkpoints --------------------------------------------------------
 
-    @torch.no_grad()
     def load_state_dict(self, state_dict):
         """Copy a state dict of this class (same ``state_bits`` and, if it keeps one, an average), or
-        one of ``torch.optim.AdamW`` for ``state_bits`` 32.  Parameters without an entry start anew."""
+        one of ``torch.optim.AdamW`` for ``state_bits`` 32.  Parameters without an entry start anew.
+        Hooks registered for loading run before (they may give another dict) and after it."""
+        state_dict = dict(state_dict)      # hooks may change its entries
+        for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
+            changed = hook(self, state_dict)
+            state_dict = state_dict if changed is None else changed
+        self._load(state_dict)
+        for hook in list(self._optimizer_load_state_dict_post_hooks.values()):
+            hook(self)
+
+    @torch.no_grad()
+    def _load(self, state_dict):
         groups, saved = state_dict["param_groups"], state_dict["state"]
         if len(groups) != len(self.param_groups) or any(len(a["params"]) != len(b["params"])
                                                         for a, b in zip(groups, self.param_groups)):

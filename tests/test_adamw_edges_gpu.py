@@ -108,3 +108,26 @@ def test_state_dicts_with_missing_entries(bits, ema, cuda_device):
     if bits == 32:      # the library's, before its first step
         opt.load_state_dict(torch.optim.AdamW(make([700, 0, 300], cuda_device), lr=0.125).state_dict())
         assert opt.param_groups[0]["lr"] == 0.125 and not opt.state[params[0]]["exp_avg"].any()
+
+
+def test_hooks_of_loading_run(cuda_device):
+    from ictc_o3.optim import AdamW
+    opt, calls = AdamW(make([300], cuda_device), lr=0.5), []
+
+    def before(optimizer, state_dict):
+        calls.append(("before", optimizer is opt, optimizer.param_groups[0]["lr"]))
+        groups = [{**g, "lr": 2 * g["lr"]} for g in state_dict["param_groups"]]
+        return {**state_dict, "param_groups": groups}
+
+    removed = opt.register_load_state_dict_pre_hook(lambda optimizer, state_dict: calls.append("removed"))
+    opt.register_load_state_dict_pre_hook(before)
+    opt.register_load_state_dict_post_hook(lambda optimizer: calls.append(("after", optimizer.param_groups[0]["lr"])))
+    removed.remove()
+    other = AdamW(make([300], cuda_device), lr=0.125)
+    other.step()
+    saved = other.state_dict()
+    opt.load_state_dict(saved)
+    assert calls == [("before", True, 0.5), ("after", 0.25)]
+    assert saved["param_groups"][0]["lr"] == 0.125          # the caller's dict is what it was
+    (p,), (q,) = opt.param_groups[0]["params"], other.param_groups[0]["params"]
+    assert torch.equal(opt.state[p]["exp_avg"], other.state[q]["exp_avg"]) and int(opt.state[p]["step"]) == 1
