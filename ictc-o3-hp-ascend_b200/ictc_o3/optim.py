@@ -26,6 +26,11 @@ def _number(value, name, low, high=math.inf, open_low=False):
     return value
 
 
+def _check_seed(seed):
+    if not isinstance(seed, int) or isinstance(seed, bool) or not 0 <= seed < 1 << 64:
+        raise ValueError("seed must be an integer in [0, 2^64)")
+
+
 def _hyperparameters(group):
     betas = group["betas"]
     if not isinstance(betas, (tuple, list)) or len(betas) != 2:
@@ -66,8 +71,7 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError("state_bits must be 8 or 32")
         if not isinstance(skip_nonfinite, bool):
             raise TypeError("skip_nonfinite must be a boolean")
-        if not isinstance(seed, int) or isinstance(seed, bool) or not 0 <= seed < 1 << 64:
-            raise ValueError("seed must be an integer in [0, 2^64)")
+        _check_seed(seed)
         self.state_bits = state_bits
         self.skip_nonfinite = skip_nonfinite
         self.seed = seed
@@ -210,9 +214,18 @@ class AdamW(torch.optim.Optimizer):
 
     # -- checkpoints --------------------------------------------------------
 
+    def state_dict(self):
+        """The base class's, and with 8-bit states the ``seed`` of their rounding; ``max_norm``,
+        ``skip_nonfinite`` and ``ema_decay`` belong to the constructor."""
+        state_dict = super().state_dict()
+        if self.state_bits == 8:
+            state_dict["seed"] = self.seed
+        return state_dict
+
     def load_state_dict(self, state_dict):
         """Copy a state dict of this class (same ``state_bits`` and, if it keeps one, an average), or
         one of ``torch.optim.AdamW`` for ``state_bits`` 32.  Parameters without an entry start anew.
+        A ``seed`` among the entries becomes this optimizer's, so that 8-bit states go on as they would have.
         Hooks registered for loading run before (they may give another dict) and after it."""
         state_dict = dict(state_dict)      # hooks may change its entries
         for hook in list(self._optimizer_load_state_dict_pre_hooks.values()):
@@ -236,6 +249,8 @@ class AdamW(torch.optim.Optimizer):
             values["lr"] = float(values["lr"])
             _hyperparameters(values)
             loaded.append(values)
+        seed = state_dict.get("seed", self.seed)
+        _check_seed(seed)
         names, exponents = [name for group in groups for name in group["params"]], []
         for name, p in zip(names, self._params):
             entry, mine = saved.get(name), self.state[p]
@@ -260,6 +275,7 @@ class AdamW(torch.optim.Optimizer):
             # other entries (a scheduler's initial_lr) come along
             group.update({k: v for k, v in theirs.items() if k != "params"}, **values)
             group["betas"] = tuple(values["betas"])
+        self.seed = seed
         steps, to, values = [], [], []
         for name, p in zip(names, self._params):
             entry, mine = saved.get(name), self.state[p]

@@ -131,3 +131,29 @@ def test_hooks_of_loading_run(cuda_device):
     assert saved["param_groups"][0]["lr"] == 0.125          # the caller's dict is what it was
     (p,), (q,) = opt.param_groups[0]["params"], other.param_groups[0]["params"]
     assert torch.equal(opt.state[p]["exp_avg"], other.state[q]["exp_avg"]) and int(opt.state[p]["step"]) == 1
+
+
+def test_seed_travels_with_8_bit_states(cuda_device):
+    """A resumed optimizer rounds as the saved one would have, whatever seed it was built with."""
+    from ictc_o3.optim import AdamW
+    params, twins = make([5000, 33], cuda_device, seed=51), make([5000, 33], cuda_device, seed=51)
+    opt, other = AdamW(params, state_bits=8, seed=(1 << 64) - 3), AdamW(twins, state_bits=8, seed=8)
+    opt.step()
+    for p, q in zip(params, twins):
+        q.data.copy_(p.data)
+    saved = opt.state_dict()
+    other.load_state_dict(saved)
+    assert other.seed == (1 << 64) - 3
+    opt.step()
+    other.step()
+    assert all(torch.equal(a, b) for a, b in zip(snapshot(opt, params), snapshot(other, twins)))
+    del saved["seed"]                 # one of an earlier release keeps the optimizer's own
+    third = AdamW(make([5000, 33], cuda_device), state_bits=8, seed=8)
+    third.load_state_dict(saved)
+    assert third.seed == 8
+    for bad in (-1, 1 << 64, 0.5, True, None):
+        kept = snapshot(other, twins)
+        with pytest.raises(ValueError, match="seed"):
+            other.load_state_dict({**saved, "state": {}, "seed": bad})
+        assert all(torch.equal(a, b) for a, b in zip(kept, snapshot(other, twins)))
+    assert "seed" not in AdamW(make([3], cuda_device)).state_dict()
