@@ -218,6 +218,8 @@ class AdamW(torch.optim.Optimizer):
         """The base class's, and with 8-bit states the ``seed`` of their rounding; ``max_norm``,
         ``skip_nonfinite`` and ``ema_decay`` belong to the constructor."""
         state_dict = super().state_dict()
+        # dicts of their own: a value replaced in the optimizer's would part it from the buffers that the kernels use
+        state_dict["state"] = {k: dict(v) for k, v in state_dict["state"].items()}
         if self.state_bits == 8:
             state_dict["seed"] = self.seed
         return state_dict

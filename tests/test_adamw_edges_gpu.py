@@ -157,3 +157,20 @@ def test_seed_travels_with_8_bit_states(cuda_device):
             other.load_state_dict({**saved, "state": {}, "seed": bad})
         assert all(torch.equal(a, b) for a, b in zip(kept, snapshot(other, twins)))
     assert "seed" not in AdamW(make([3], cuda_device)).state_dict()
+
+
+def test_edited_state_dicts_load(cuda_device):
+    """Values replaced in a state dict change the optimizer when it is loaded, and not before."""
+    from ictc_o3.optim import AdamW
+    (p,) = params = make([700], cuda_device, seed=61)
+    opt = AdamW(params, **HYPER, ema_decay=0.9)
+    opt.step()
+    saved, m = opt.state_dict(), opt.state[p]["exp_avg"].clone()
+    saved["state"][0]["ema"] = torch.full((700,), 2.0, device=cuda_device)
+    saved["state"][0]["exp_avg"] = 3 * m
+    assert torch.equal(opt.state[p]["exp_avg"], m)
+    opt.load_state_dict(saved)
+    assert torch.equal(opt.state[p]["exp_avg"], 3 * m) and torch.equal(opt.moments()[0][:700], 3 * m)
+    assert bool((opt.averages()[:700] == 2.0).all())
+    opt.step()
+    assert torch.equal(opt.state[p]["ema"], opt.averages()[:700]) and bool((opt.averages()[:700] != 2.0).any())
