@@ -58,16 +58,18 @@ static_assert(kTurn == kThreads * kQuads * 4 && kBlockValues == 32 * kQuads * 4,
 
 // A tensor's bias corrections for its next step, left behind by the last one: a block then reads
 // them with its values instead of waiting for one thread's FP64 exponentials (8-bit states, 160 M
-// values: 820 -> 716 us).  They hold for the step number and betas they name, else they are made again.
+// values: 820 -> 716 us).  They hold for the step number and betas they name, else they are made again: betas by
+// their FP64 logarithms, since betas near 1 that FP32 cannot tell apart may differ by a tenth of 1 - b.
 struct alignas(32) Rate {
   float m;        // 1 / (1 - b1^t)
   float v;        // 1 / sqrt(1 - b2^t)
-  float b1, b2;
+  double log_b1, log_b2;
   int64_t t;
 };
 
-__device__ __forceinline__ Rate rate_of(int64_t t, double log_b1, double log_b2, float b1, float b2) {
-  return Rate{(float)(1.0 / -expm1((double)t * log_b1)), (float)(1.0 / sqrt(-expm1((double)t * log_b2))), b1, b2, t};
+__device__ __forceinline__ Rate rate_of(int64_t t, double log_b1, double log_b2) {
+  return Rate{(float)(1.0 / -expm1((double)t * log_b1)), (float)(1.0 / sqrt(-expm1((double)t * log_b2))), log_b1, log_b2,
+              t};
 }
 
 // Caller-owned device words, zeroed once.  The tickets count finished blocks and return
@@ -430,7 +432,7 @@ adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
     const int64_t t = a.steps[c.x] + 1;
     Rate rate = a.rates[c.x];
     const float clip = a.use_norm ? a.ws->clip : 1.f;
-    if (rate.t != t || rate.b1 != a.b1 || rate.b2 != a.b2) rate = rate_of(t, a.log_b1, a.log_b2, a.b1, a.b2);
+    if (rate.t != t || rate.log_b1 != a.log_b1 || rate.log_b2 != a.log_b2) rate = rate_of(t, a.log_b1, a.log_b2);
     const float size = a.lr * rate.m;
 #pragma unroll 1
     for (int k = 0; k < mine; ++k) {
@@ -475,7 +477,7 @@ adamw_kernel(const __grid_constant__ TensorList list, const Args a) {
         if (list.t[i].grad != nullptr) {
           const int64_t t = a.steps[a.tensor0 + i] + 1;
           a.steps[a.tensor0 + i] = t;
-          a.rates[a.tensor0 + i] = rate_of(t + 1, a.log_b1, a.log_b2, a.b1, a.b2);
+          a.rates[a.tensor0 + i] = rate_of(t + 1, a.log_b1, a.log_b2);
         }
     if (threadIdx.x == 0) a.ws->step_ticket = 0;
   }

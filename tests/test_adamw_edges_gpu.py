@@ -174,3 +174,24 @@ def test_edited_state_dicts_load(cuda_device):
     assert bool((opt.averages()[:700] == 2.0).all())
     opt.step()
     assert torch.equal(opt.state[p]["ema"], opt.averages()[:700]) and bool((opt.averages()[:700] != 2.0).any())
+
+
+@pytest.mark.parametrize("before, after", [((0.9, 0.9999999), (0.9, 0.99999991)), ((0.99999991, 0.99), (0.9999999, 0.99)),
+                                           ((0.0, 0.99), (0.9, 0.0))])
+def test_betas_that_fp32_cannot_tell_apart(before, after, cuda_device):
+    """Bias corrections left behind by a step hold for its own betas only."""
+    from ictc_o3.optim import AdamW
+    params, twins = make([700, 33], cuda_device, seed=71), make([700, 33], cuda_device, seed=71)
+    opt = AdamW(params, lr=0.1, betas=before)
+    opt.step()
+    for p, q in zip(params, twins):
+        q.data.copy_(p.data)
+    fresh = AdamW(twins, lr=0.1, betas=before)
+    fresh.load_state_dict(opt.state_dict())              # copies no bias corrections
+    for o in (opt, fresh):
+        o.param_groups[0]["betas"] = after
+        o.step()
+    assert all(torch.equal(p, q) for p, q in zip(params, twins))
+    for p, q in zip(params, twins):
+        for k in ("exp_avg", "exp_avg_sq"):
+            assert torch.equal(opt.state[p][k], fresh.state[q][k])
