@@ -113,7 +113,7 @@ struct Args {
   float b1, c1, b2, c2;      // betas and 1 - beta
   float lr, eps, keep;       // keep = 1 - lr wd
   // The average as a step of `share` from one value towards the other (d and 1 - d rounded by themselves do not
-  // add up to one: at d = 0.9999 an average of equal weights would drift by 1.7e-4 of them); nearer: share = d, from
+  // add up to one: at d = 0.9999 an average of equal weights would drift by 1.7e-4 of them); nearer: share = -d, from
   // the new weight, so that d = 0 gives the weight itself, else share = 1 - d, from the old average.
   float share;
   int nearer;
@@ -388,10 +388,7 @@ __device__ __forceinline__ void update(const Turn<BITS, AVERAGE>& x, const Args&
     if constexpr (AVERAGE) {
       float e[4] = {x.e[q].x, x.e[q].y, x.e[q].z, x.e[q].w};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float from = a.nearer ? w[q][i] : e[i], to = a.nearer ? e[i] : w[q][i];
-        e[i] = fmaf(a.share, __fsub_rn(to, from), from);
-      }
+      for (int i = 0; i < 4; ++i) e[i] = fmaf(a.share, __fsub_rn(w[q][i], e[i]), a.nearer ? w[q][i] : e[i]);
       *reinterpret_cast<float4*>(a.average + s0 + q * 128) = make_float4(e[0], e[1], e[2], e[3]);
     }
   }
@@ -602,7 +599,7 @@ extern "C" int ictc_adamw_step(void* const* weights, const void* const* grads, i
   a.eps = (float)eps;
   a.keep = (float)(1.0 - lr * weight_decay);
   a.nearer = average_decay < 0.5;
-  a.share = (float)(a.nearer ? average_decay : 1.0 - average_decay);
+  a.share = (float)(a.nearer ? -average_decay : 1.0 - average_decay);
   a.lr = (float)lr;
   a.log_b1 = log(beta1);
   a.log_b2 = log(beta2);
