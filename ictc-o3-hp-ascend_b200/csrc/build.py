@@ -4,7 +4,8 @@ Each .cu file is compiled to an object in parallel, then linked into
 ``ictc_o3/backends/cuda/libictc_cuda.so`` beside the Python package that
 loads it.  The CUDA runtime is linked statically, so the library carries no
 dependency on a particular libcudart soname.  host_tensors.cpp becomes a Python
-extension module beside it (g++, against the installed torch and this interpreter).
+extension module beside it (g++, against the installed torch and this interpreter);
+where that fails, the package runs without it.
 
     python build.py [--force] [--verbose]
 """
@@ -81,7 +82,18 @@ def build_host(force=False):
 
 def build(force=False, verbose=False):
     os.makedirs(OBJDIR, exist_ok=True)
-    build_host(force)
+    output = build_kernels(force, verbose)
+    try:
+        build_host(force)
+    except (RuntimeError, OSError) as error:      # no g++, or no headers of Python or torch: slower, not unusable
+        if os.path.exists(HOST_OUTPUT):
+            os.remove(HOST_OUTPUT)
+        sys.stderr.write(f"{error}\nwithout _host_tensors the optimizer reads its tensors' addresses in Python and "
+                         "block norms refuse captured backward passes\n")
+    return output
+
+
+def build_kernels(force=False, verbose=False):
     srcs = sources()
     with concurrent.futures.ThreadPoolExecutor(max_workers=max(1, min(len(srcs), os.cpu_count() or 1))) as pool:
         objs = list(pool.map(lambda s: _compile(s, force, verbose), srcs))

@@ -195,3 +195,30 @@ def test_betas_that_fp32_cannot_tell_apart(before, after, cuda_device):
     for p, q in zip(params, twins):
         for k in ("exp_avg", "exp_avg_sq"):
             assert torch.equal(opt.state[p][k], fresh.state[q][k])
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_without_the_extension_module(bits, cuda_device, monkeypatch):
+    """Where it was not built, addresses and checks go through Python, with the same results and refusals."""
+    from ictc_o3.backends.cuda import _native
+    from ictc_o3.optim import AdamW
+    sets = [make([5000, 0, 33, 7], cuda_device, seed=81) for _ in range(2)]
+    opts = [AdamW(sets[0], state_bits=bits, max_norm=1.0, ema_decay=0.9)]
+
+    def missing():
+        raise _native.NativeError("not built")
+
+    monkeypatch.setattr(_native, "host_tensors", missing)
+    opts.append(AdamW(sets[1], state_bits=bits, max_norm=1.0, ema_decay=0.9))
+    for params in sets:
+        params[3].grad = None
+    versions = [p._version for p in sets[1]]
+    for _ in range(2):
+        for opt in opts:
+            opt.step()
+    assert all(torch.equal(a, b) for a, b in zip(*(snapshot(o, p) for o, p in zip(opts, sets))))
+    assert [p._version > v for p, v in zip(sets[1], versions)] == [True, True, True, False]
+    sets[1][0].data = torch.zeros(5, device=cuda_device)
+    sets[1][0].grad = torch.zeros(5, device=cuda_device)
+    with pytest.raises(ValueError, match="has changed"):
+        opts[1].step()
