@@ -64,12 +64,15 @@ def build_host(force=False):
     except ImportError:
         return None
     root = os.path.dirname(os.path.abspath(torch.__file__))
-    stamp = max(os.path.getmtime(HOST_SOURCE), os.path.getmtime(os.path.join(root, "version.py")))
-    if not force and os.path.exists(HOST_OUTPUT) and os.path.getmtime(HOST_OUTPUT) >= stamp:
+    # times of installed files say nothing: an older torch may be installed later
+    built_for, stamp = f"{torch.__version__}\n{root}\n", os.path.join(OBJDIR, "host_tensors.torch")
+    if (not force and os.path.exists(HOST_OUTPUT) and os.path.exists(stamp) and open(stamp).read() == built_for
+            and os.path.getmtime(HOST_OUTPUT) >= os.path.getmtime(HOST_SOURCE)):
         return HOST_OUTPUT
     tmp = HOST_OUTPUT + ".tmp"
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           f'-DICTC_TORCH_VERSION="{torch.__version__}"',
            "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
            "-I" + sysconfig.get_paths()["include"], HOST_SOURCE, "-L" + os.path.join(root, "lib"),
            "-lc10", "-ltorch_cpu", "-ltorch_python", "-o", tmp]
@@ -77,6 +80,8 @@ def build_host(force=False):
     if proc.returncode != 0:
         raise RuntimeError(f"g++ failed for host_tensors.cpp:\n{proc.stderr}")
     os.replace(tmp, HOST_OUTPUT)
+    with open(stamp, "w") as f:
+        f.write(built_for)
     return HOST_OUTPUT
 
 

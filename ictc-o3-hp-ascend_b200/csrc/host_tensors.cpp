@@ -115,4 +115,12 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_host_tensors", nullptr, -1, metho
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit__host_tensors() { return PyModule_Create(&module); }
+// torch_version: the torch whose structures this file was compiled for; with another one it must not be used.
+PyMODINIT_FUNC PyInit__host_tensors() {
+  PyObject* self = PyModule_Create(&module);
+  if (self && PyModule_AddStringConstant(self, "torch_version", ICTC_TORCH_VERSION) < 0) {
+    Py_DECREF(self);
+    return nullptr;
+  }
+  return self;
+}

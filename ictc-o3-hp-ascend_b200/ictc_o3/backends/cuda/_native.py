@@ -135,6 +135,9 @@ def host_tensors():
     except ImportError as error:
         raise NativeError(f"_host_tensors is missing or was built for another torch ({error}); "
                           "run __graft_entry__.build()") from error
+    if getattr(_host_tensors, "torch_version", None) != str(torch.__version__):      # it reads torch's own structures
+        raise NativeError(f"_host_tensors was built for another torch than {torch.__version__}; "
+                          "run __graft_entry__.build()")
     return _host_tensors
 
 

@@ -47,3 +47,26 @@ def test_a_kernel_that_does_not_compile_ends_the_build(builder):
     builder.fails["nvcc"] = "error"
     with pytest.raises(RuntimeError, match="nvcc"):
         builder.build()
+
+
+def test_the_extension_module_is_built_again_for_another_torch(builder, monkeypatch):
+    """Whatever the installed files' times: an older torch may be installed after a newer one."""
+    import torch
+    builds = lambda: [t for t, _ in builder.ran].count("g++")  # noqa: E731
+    for k in (1, 1):
+        builder.build()
+        assert builds() == k and os.path.exists(builder.HOST_OUTPUT)
+    monkeypatch.setattr(torch, "__version__", "2.0.0")
+    builder.build()
+    builder.build()
+    assert builds() == 2
+    assert any("2.0.0" in x for x in builder.ran[-1][1] if x.startswith("-DICTC"))
+
+
+def test_an_extension_module_for_another_torch_is_not_used(monkeypatch):
+    import torch
+    from ictc_o3.backends.cuda import _native
+    assert _native.host_tensors().torch_version == torch.__version__
+    monkeypatch.setattr(torch, "__version__", "2.0.0")
+    with pytest.raises(_native.NativeError, match="another torch"):
+        _native.host_tensors()
