@@ -95,8 +95,8 @@ class AdamW(torch.optim.Optimizer):
             _hyperparameters(group)
         params = [p for group in self.param_groups for p in group["params"]]
         require_cuda_fp32(*params)
-        if any(not p.is_contiguous() for p in params):
-            raise ValueError("the optimizer requires contiguous parameters")
+        if any(not p.is_contiguous() or p.is_neg() for p in params):
+            raise ValueError("the optimizer requires contiguous parameters that are no lazily negated views")
         spans = sorted((p.data_ptr(), 4 * p.numel()) for p in params if p.numel())
         if len({id(p) for p in params}) != len(params) or any(a + n > b for (a, n), (b, _) in zip(spans, spans[1:])):
             raise ValueError("parameters must not repeat or share memory")
@@ -156,7 +156,8 @@ class AdamW(torch.optim.Optimizer):
         for i, (p, g, size) in enumerate(zip(self._params, kept, self._sizes)):
             if g is None:
                 continue
-            if p.dtype is not torch.float32 or p.device != self._device or p.numel() != size or not p.is_contiguous():
+            if (p.dtype is not torch.float32 or p.device != self._device or p.numel() != size or not p.is_contiguous()
+                    or p.is_neg()):
                 raise ValueError("a parameter has changed its type, device, size or layout since the optimizer was built")
             if (g.layout is not torch.strided or g.dtype is not torch.float32 or g.device != self._device
                     or g.numel() != size):

@@ -222,3 +222,17 @@ def test_without_the_extension_module(bits, cuda_device, monkeypatch):
     sets[1][0].grad = torch.zeros(5, device=cuda_device)
     with pytest.raises(ValueError, match="has changed"):
         opts[1].step()
+
+
+def test_negated_parameters_are_refused(cuda_device):
+    """A lazily negated view stores the other sign: steps would go uphill."""
+    from ictc_o3.optim import AdamW
+    negated = torch._neg_view(torch.ones(5, device=cuda_device))
+    with pytest.raises(ValueError, match="negated"):
+        AdamW([torch.nn.Parameter(negated)])
+    p = torch.nn.Parameter(torch.ones(5, device=cuda_device))
+    opt = AdamW([p])
+    p.data = negated
+    p.grad = torch.ones(5, device=cuda_device)
+    with pytest.raises(ValueError, match="has changed"):
+        opt.step()
