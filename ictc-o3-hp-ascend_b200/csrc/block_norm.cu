@@ -84,6 +84,8 @@ bool shape_of(int C, int L, int mode, unsigned there, bool sums, int64_t rows, i
   return false;
 }
 
+std::atomic<uint64_t> wait_limit{kWaitNs};
+
 int invalid(const char* what) {
   ictc_set_error(what, "");
   return ICTC_ERR_INVALID;
@@ -113,6 +115,7 @@ int run(int mode, BlockArgs& a, int lmax, int layout, bool branch, int* blocks, 
     ictc_set_error("ictc_block: rows of this width do not fit shared memory%s", "");
     return ICTC_ERR_UNSUPPORTED;
   }
+  a.wait_ns = wait_limit.load(std::memory_order_relaxed);
   a.wide = 0;
   a.row_bytes = 0;
   s.bulk = s.hold && s.stages > 1;
@@ -169,6 +172,12 @@ bool bad_shape(int64_t rows, int channels, int lmax, int layout, float eps) {
 
 using namespace ictc;
 using namespace ictc::block_norm;
+
+extern "C" int ictc_block_wait_limit(uint64_t nanoseconds) {
+  if (nanoseconds > kWaitNs) return invalid("ictc_block_wait_limit: at most two seconds%s");
+  wait_limit.store(nanoseconds, std::memory_order_relaxed);
+  return ICTC_OK;
+}
 
 extern "C" int64_t ictc_block_partial_floats(int channels, int lmax) {
   if (channels < 1 || lmax < 0 || lmax > kMaxL) return -1;

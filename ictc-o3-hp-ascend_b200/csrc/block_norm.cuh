@@ -96,7 +96,7 @@ __host__ __device__ constexpr int max_row_warps(int mode, int L) {
 }
 constexpr int kScratch = 16;                          // sums of one warp
 constexpr int kBarrierFloats = 8;                     // room of four mbarriers
-constexpr uint64_t kWaitNs = 2000000000ull;           // a copy that takes longer is given up
+constexpr uint64_t kWaitNs = 2000000000ull;           // BlockArgs::wait_ns, unless a test shortens it; limit of draining
 
 struct BlockArgs {
   const float* in[kSlots];  // null: zeros, or not there
@@ -108,6 +108,7 @@ struct BlockArgs {
   const float* scale;
   const float* pre;
   int* status;              // 1 (3) after a copy did not land in time (nor while draining)
+  uint64_t wait_ns;         // a copy that takes longer is given up; 0: every copy is, unseen
   float* r1_out;            // [N, 4], or null (forward)
   float* r2_out;
   float* partial;           // [blocks][2][(L+1) C] weight-gradient sums, or null
@@ -378,18 +379,12 @@ __global__ void __launch_bounds__(32 * max_warps(MODE, L)) block_kernel(const __
   for (int s = 0; s + 1 < a.stages; ++s) fetch(first + s * stride, s);
   int stage = 0, waited = 0;
   uint32_t parity = 0;
-  for (int64_t t = first; t < tiles; t += stride) {
+  int64_t t = first;
+  for (; t < tiles; t += stride) {
     if constexpr (BULK) {
-      const bool landed = g.sync_all(g.thread != 0 || tc::mbar_wait(full + stage, parity, kWaitNs));
-      if (!landed) {      // report, let the copies in flight end, and leave
-        if (g.thread == 0) {
-          bool drained = true;
-          for (int j = waited; j < issued; ++j)
-            drained = tc::mbar_wait(full + j % a.stages, (j / a.stages) & 1, kWaitNs) && drained;
-          atomicMax(a.status, drained ? 1 : 3);
-        }
-        break;
-      }
+      const bool landed =
+          g.sync_all(g.thread != 0 || (a.wait_ns != 0 && tc::mbar_wait(full + stage, parity, a.wait_ns)));
+      if (!landed) break;
       ++waited;
     } else if (a.stages == 1) {
       g.sync();
@@ -736,7 +731,38 @@ __global__ void __launch_bounds__(32 * max_warps(MODE, L)) block_kernel(const __
     }
     stage = stage + 1 == a.stages ? 0 : stage + 1;
   }
-  if (BULK && g.thread == 0) bulk_read_wait();      // shared memory outlives the stores that read it
+  if constexpr (BULK) {
+    // A copy did not land in time: report it, let those in flight end, and leave NaN in all rows that are
+    // left and in the weights' gradients (unwritten memory could pass for a result).
+    if (t < tiles) {
+      if (g.thread == 0) {
+        bool drained = true;
+        for (int j = waited; j < issued; ++j)
+          drained = tc::mbar_wait(full + j % a.stages, (j / a.stages) & 1, kWaitNs) && drained;
+        atomicMax(a.status, drained ? 1 : 3);
+      }
+      const float nan = __int_as_float(0x7fffffff);
+#pragma unroll 1
+      for (; t < tiles; t += stride) {
+        const int64_t row0 = t * a.per;
+        const int rows = (int)(a.rows - row0 < a.per ? a.rows - row0 : a.per);
+        // (the loop's form moves the registers of the code before it: rolled, the norm alone takes 53 us instead of 49
+        // for 50,000 rows of C132/lmax 1; unrolled, the forward with a branch 93 us instead of 91)
+#pragma unroll (BRANCH ? 1 : 9)
+        for (int s = 0; s < 9; ++s) {
+          float* to = s < 6 ? a.out[s] : s == 6 ? a.gate_out : s == 7 ? a.r1_out : a.r2_out;
+          const int wd = s < 6 ? W : s == 6 ? width : 4;
+          if (to == nullptr) continue;
+#pragma unroll 1
+          for (int i = g.thread; i < rows * wd; i += g.threads) to[row0 * wd + i] = nan;
+        }
+      }
+      if constexpr (MODE != kForward) {
+        ICTC_DEGREES(l, N) sum_w[l] = sum_b[l] = nan;
+      }
+    }
+    if (g.thread == 0) bulk_read_wait();      // shared memory outlives the stores that read it
+  }
   if (a.partial == nullptr) return;
   // Sums of the block's groups (and of a warp's rows side by side), in order.
   __syncthreads();

@@ -63,15 +63,20 @@ def _check(form, rows, weights, gate=None):
         raise ValueError("Gates must have shape [N,(L+1)*C] or [N,L+1,C]")
 
 
-def block_norm_status(device="cuda"):
+def block_norm_status(device="cuda", reset=False):
     """0, or what a kernel of this module left after a copy into shared memory did not land within two
-    seconds (its results are then not valid).  Reads one int from the device: for tests and after a step."""
+    seconds; the results that it could not compute are NaN then.  Reads one int from the device, and with
+    ``reset`` clears it: for tests, or to tell the cause of NaN."""
     device = torch.device(device)
     if device.type != "cuda":
         raise ValueError("block norms run on CUDA devices")
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    return int(status_word(device))
+    word = status_word(device)
+    value = int(word)
+    if reset:
+        word.zero_()
+    return value
 
 
 def degree_norm(features, weight=None, *, channels, lmax, layout="mul_ir", eps=1e-6):

@@ -406,7 +406,9 @@ int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_scale, cons
  * (16-byte aligned; the first L+1 count) receive r(branch) and r of the normed rows
  * (NULL: not kept); the derivatives read them.  status: a device int, zeroed by the
  * caller, that becomes 1 when rows did not arrive in shared memory within two seconds
- * and the kernel left its work undone (3: the copy may still be in flight).
+ * and the kernel left its work undone (3: the copy may still be in flight); the results
+ * that it left out are NaN then.  ictc_block_wait_limit sets that time for later launches
+ * of the process (2e9 ns at most; 0: every wait runs out), for tests of such an end.
  *
  * ictc_block_backward: gradients for the cotangents p of stream_out and q of normed
  * (either may be NULL: zero; q = NULL means no norm took part, the gradient of stream
@@ -421,6 +423,7 @@ int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_scale, cons
  */
 int64_t ictc_block_partial_floats(int channels, int lmax);
 int ictc_block_supported(int channels, int lmax);
+int ictc_block_wait_limit(uint64_t nanoseconds);
 int ictc_block_forward(const float* stream_in, const float* branch, const float* gate, const float* post,
                        const float* scale, const float* pre, int norm, int64_t rows, int channels, int lmax,
                        int layout, float eps, float* stream_out, float* normed, float* r1, float* r2, int* status,

@@ -29,3 +29,10 @@ def test_launches_take_no_host_tensors(monkeypatch):
     with pytest.raises(TypeError, match="CUDA tensors"):
         _native.launch(torch.device("cuda", 0), "ictc_block_forward", torch.tensor(3))
     assert len(called) == 1
+
+
+def test_wait_limit_has_a_bound():
+    from ictc_o3.backends.cuda import _native
+    lib = _native.library()
+    assert lib.ictc_block_wait_limit(2_000_000_001) == -1 and "two seconds" in lib.ictc_last_error().decode()
+    assert lib.ictc_block_wait_limit(2_000_000_000) == 0

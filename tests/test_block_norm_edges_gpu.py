@@ -1,4 +1,6 @@
 """Block norms with tensors and calls out of the ordinary."""
+import contextlib
+
 import pytest
 import torch
 
@@ -67,3 +69,51 @@ def test_forward_mode_over_a_backward_pass_is_refused(second, cuda_device):
         cotangents[0] = forward_ad.make_dual(cotangents[0].detach(), torch.ones_like(cotangents[0]))
         with pytest.raises(ValueError, match="forward-mode"):
             torch.autograd.grad(out, [t["branch"], t["scale"]], cotangents)
+
+
+@contextlib.contextmanager
+def no_patience():
+    """Every wait of the block norms for a copy runs out at once (the kernels then drain their copies)."""
+    from ictc_o3.backends.cuda import _native
+    try:
+        _native.call("ictc_block_wait_limit", 0)
+        yield
+    finally:
+        torch.cuda.synchronize()
+        _native.call("ictc_block_wait_limit", 2_000_000_000)
+
+
+@pytest.mark.parametrize("n, channels, lmax", [(1, 64, 2), (37, 4, 0), (301, 8, 3), (20_011, 8, 1), (900, 128, 3), (2003, 132, 1)])
+def test_given_up_copies_leave_nan(n, channels, lmax, cuda_device):
+    """A kernel whose rows did not arrive reports it, leaves NaN in what it did not compute, and the next
+    one works again."""
+    from ictc_o3.ops.block_norm import block_norm_status, residual_block_norm
+    t = inputs(n, channels, lmax)
+    leaves = [t[k] for k in NAMES]
+
+    def forward():
+        return residual_block_norm(t["stream"], t["branch"], **{k: t[k] for k in NAMES[2:]}, channels=channels, lmax=lmax)
+
+    def first(out):
+        return torch.autograd.grad(out, leaves, [t["p"], t["q"]], create_graph=True)
+
+    def second(grads):
+        return torch.autograd.grad(grads[:3], [*leaves, t["p"], t["q"]], [t["d_stream"], t["d_branch"], t["d_gate"]],
+                                   retain_graph=True)
+
+    def spoilt(results):
+        code = block_norm_status(reset=True)
+        return code == 1 and all(bool(x.isnan().all()) for x in results)
+
+    out = forward()
+    grads = first(out)
+    want = [x.detach().clone() for x in (*out, *grads, *second(grads))]
+    assert block_norm_status() == 0
+    with no_patience():
+        assert spoilt(forward())
+        assert spoilt(first(out))
+        assert spoilt(second(grads))
+    again = forward()
+    grads = first(again)
+    assert all(torch.equal(a, b) for a, b in zip((*again, *grads, *second(grads)), want))
+    assert block_norm_status() == 0
