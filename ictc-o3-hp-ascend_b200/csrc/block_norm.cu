@@ -5,6 +5,10 @@ namespace ictc {
 namespace block_norm {
 namespace {
 
+// The status word of callers without one of their own, per device.  The library's memory and not an allocation: it is
+// there, zeroed, before any stream captures, and graphs may keep its address.
+__device__ int own_status;
+
 // Weight gradients from the blocks' sums: one warp per (degree, channel) column.
 __global__ void __launch_bounds__(256) weight_sum_kernel(const float* __restrict__ partial, int blocks, int columns,
                                                          const float* __restrict__ post,
@@ -91,6 +95,12 @@ int invalid(const char* what) {
   return ICTC_ERR_INVALID;
 }
 
+int checked(cudaError_t err) {
+  if (err == cudaSuccess) return ICTC_OK;
+  ictc_set_error("ictc_block: %s", cudaGetErrorString(err));
+  return ICTC_ERR_CUDA;
+}
+
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
 int sm_count() {
@@ -141,11 +151,7 @@ int run(int mode, BlockArgs& a, int lmax, int layout, bool branch, int* blocks, 
   const cudaError_t err = mode == kForward    ? launch_forward(a, s, grid, bytes, lmax, layout, branch, stream)
                           : mode == kBackward ? launch_backward(a, s, grid, bytes, lmax, layout, branch, stream)
                                               : launch_second(a, s, grid, bytes, lmax, layout, branch, stream);
-  if (err != cudaSuccess) {
-    ictc_set_error("ictc_block: %s", cudaGetErrorString(err));
-    return ICTC_ERR_CUDA;
-  }
-  return ICTC_OK;
+  return checked(err);
 }
 
 int weight_sums(const BlockArgs& a, int lmax, int blocks, float* grad_post, float* grad_scale, float* grad_pre,
@@ -153,12 +159,7 @@ int weight_sums(const BlockArgs& a, int lmax, int blocks, float* grad_post, floa
   const int columns = (lmax + 1) * a.channels;
   weight_sum_kernel<<<(columns + 7) / 8, 256, 0, stream>>>(a.partial, blocks, columns, a.post, a.scale, grad_post,
                                                            grad_scale, grad_pre);
-  cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) {
-    ictc_set_error("ictc_block: %s", cudaGetErrorString(err));
-    return ICTC_ERR_CUDA;
-  }
-  return ICTC_OK;
+  return checked(cudaGetLastError());
 }
 
 bool bad_shape(int64_t rows, int channels, int lmax, int layout, float eps) {
@@ -172,6 +173,22 @@ bool bad_shape(int64_t rows, int channels, int lmax, int layout, float eps) {
 
 using namespace ictc;
 using namespace ictc::block_norm;
+
+extern "C" int ictc_block_status_word(int** word) {
+  if (!word) return invalid("ictc_block_status_word: invalid argument%s");
+  return checked(cudaGetSymbolAddress(reinterpret_cast<void**>(word), own_status));
+}
+
+extern "C" int ictc_block_status(int reset, int* value, void* stream) {
+  if (!value) return invalid("ictc_block_status: invalid argument%s");
+  int* word = nullptr;
+  if (int rc = ictc_block_status_word(&word)) return rc;
+  cudaStream_t s = (cudaStream_t)stream;
+  if (int rc = checked(cudaMemcpyAsync(value, word, sizeof(int), cudaMemcpyDeviceToHost, s))) return rc;
+  if (reset)
+    if (int rc = checked(cudaMemsetAsync(word, 0, sizeof(int), s))) return rc;
+  return checked(cudaStreamSynchronize(s));
+}
 
 extern "C" int ictc_block_wait_limit(uint64_t nanoseconds) {
   if (nanoseconds > kWaitNs) return invalid("ictc_block_wait_limit: at most two seconds%s");

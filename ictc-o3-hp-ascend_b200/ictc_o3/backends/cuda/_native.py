@@ -68,6 +68,8 @@ _SIGNATURES = {
     "ictc_block_partial_floats": [_i, _i],
     "ictc_block_supported": [_i, _i],
     "ictc_block_wait_limit": [_u64],
+    "ictc_block_status_word": [_p],
+    "ictc_block_status": [_i, _p, _p],
     "ictc_block_forward": [_p] * 6 + [_i, _i64, _i, _i, _i, _f] + [_p] * 6,
     "ictc_block_backward": [_p] * 10 + [_i64, _i, _i, _i] + [_p] * 9,
     "ictc_block_second": [_p] * 13 + [_i64, _i, _i, _i] + [_p] * 11,

@@ -7,6 +7,7 @@ a block (``branch`` None) is the same pair.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -101,13 +102,21 @@ _status = {}
 
 
 def status_word(device):
-    """The device word (int32) that the kernels set when a copy did not land in time."""
+    """Address of the device word (int32) that the kernels set when a copy did not land in time: the
+    library's own, so captured launches set it too."""
     word = _status.get(device)
     if word is None:
-        word = torch.zeros(1, dtype=torch.int32, device=device)
-        if not torch.cuda.is_current_stream_capturing():      # a capture's memory is its graph's own
-            _status[device] = word
+        found = ctypes.c_void_p()
+        with torch.cuda.device(device):
+            _native.call("ictc_block_status_word", ctypes.byref(found))
+        word = _status[device] = found.value
     return word
+
+
+def read_status(device, reset):
+    value = ctypes.c_int()
+    launch(device, "ictc_block_status", reset, ctypes.addressof(value))
+    return value.value
 
 
 def dense(x):

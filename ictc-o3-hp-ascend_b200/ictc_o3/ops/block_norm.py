@@ -22,7 +22,7 @@ import functools
 import torch
 
 from ictc_o3.backends.cuda import _native
-from ictc_o3.backends.cuda.block_norm import LAYOUTS, Form, block, dense, status_word
+from ictc_o3.backends.cuda.block_norm import LAYOUTS, Form, block, dense, read_status
 from ictc_o3.backends.cuda.runtime import require_cuda_fp32
 
 __all__ = ["degree_norm", "residual_block_norm", "DegreeNorm", "ResidualBlockNorm",
@@ -65,18 +65,16 @@ def _check(form, rows, weights, gate=None):
 
 def block_norm_status(device="cuda", reset=False):
     """0, or what a kernel of this module left after a copy into shared memory did not land within two
-    seconds; the results that it could not compute are NaN then.  Reads one int from the device, and with
-    ``reset`` clears it: for tests, or to tell the cause of NaN."""
+    seconds; the results that it could not compute are NaN then.  Launches of replayed graphs count.  Waits
+    for the current stream, and with ``reset`` clears the word: for tests, or to tell the cause of NaN."""
     device = torch.device(device)
     if device.type != "cuda":
         raise ValueError("block norms run on CUDA devices")
     if device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    word = status_word(device)
-    value = int(word)
-    if reset:
-        word.zero_()
-    return value
+    if not isinstance(reset, bool):
+        raise TypeError("reset must be a boolean")
+    return read_status(device, reset)
 
 
 def degree_norm(features, weight=None, *, channels, lmax, layout="mul_ir", eps=1e-6):

@@ -407,7 +407,10 @@ int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_scale, cons
  * (NULL: not kept); the derivatives read them.  status: a device int, zeroed by the
  * caller, that becomes 1 when rows did not arrive in shared memory within two seconds
  * and the kernel left its work undone (3: the copy may still be in flight); the results
- * that it left out are NaN then.  ictc_block_wait_limit sets that time for later launches
+ * that it left out are NaN then.  ictc_block_status_word gives the address of a word of
+ * the library's own on the current device, zeroed when the library is loaded;
+ * ictc_block_status reads it behind the work on `stream`, clears it if asked to, and
+ * waits for both.  ictc_block_wait_limit sets that time for later launches
  * of the process (2e9 ns at most; 0: every wait runs out), for tests of such an end.
  *
  * ictc_block_backward: gradients for the cotangents p of stream_out and q of normed
@@ -424,6 +427,8 @@ int ictc_adamw_decode(const void* m, const void* v, const uint8_t* m_scale, cons
 int64_t ictc_block_partial_floats(int channels, int lmax);
 int ictc_block_supported(int channels, int lmax);
 int ictc_block_wait_limit(uint64_t nanoseconds);
+int ictc_block_status_word(int** word);
+int ictc_block_status(int reset, int* value, void* stream);
 int ictc_block_forward(const float* stream_in, const float* branch, const float* gate, const float* post,
                        const float* scale, const float* pre, int norm, int64_t rows, int channels, int lmax,
                        int layout, float eps, float* stream_out, float* normed, float* r1, float* r2, int* status,

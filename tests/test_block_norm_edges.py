@@ -31,8 +31,9 @@ def test_launches_take_no_host_tensors(monkeypatch):
     assert len(called) == 1
 
 
-def test_wait_limit_has_a_bound():
+def test_status_and_wait_limit_are_checked():
     from ictc_o3.backends.cuda import _native
     lib = _native.library()
     assert lib.ictc_block_wait_limit(2_000_000_001) == -1 and "two seconds" in lib.ictc_last_error().decode()
     assert lib.ictc_block_wait_limit(2_000_000_000) == 0
+    assert lib.ictc_block_status_word(None) == -1 and lib.ictc_block_status(0, None, None) == -1

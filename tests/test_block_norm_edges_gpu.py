@@ -117,3 +117,48 @@ def test_given_up_copies_leave_nan(n, channels, lmax, cuda_device):
     grads = first(again)
     assert all(torch.equal(a, b) for a, b in zip((*again, *grads, *second(grads)), want))
     assert block_norm_status() == 0
+
+
+def test_status_of_a_first_call_inside_a_capture(cuda_device, monkeypatch):
+    """Replays report to the word that block_norm_status reads, whether or not a call came before the capture."""
+    from ictc_o3.backends.cuda import block_norm
+    from ictc_o3.ops.block_norm import block_norm_status
+    t = {k: v.detach() for k, v in inputs(50, 12, 2).items()}
+    want = call(t)
+    assert block_norm_status() == 0
+    monkeypatch.setattr(block_norm, "_status", {})
+    graph = torch.cuda.CUDAGraph()
+    with no_patience(), torch.cuda.graph(graph):
+        held = call(t)
+    assert block_norm_status() == 0
+    for _ in range(2):
+        graph.replay()
+        assert block_norm_status(reset=True) == 1 and all(bool(x.isnan().all()) for x in held)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(call(t), want)) and block_norm_status(reset=True) == 1
+    assert block_norm_status() == 0
+    with pytest.raises(TypeError):
+        block_norm_status(reset=1)
+
+
+def test_first_use_of_the_library_inside_a_capture(cuda_device):
+    """In a process of its own: not even the library's code is on the device before the capture."""
+    import os
+    import subprocess
+    import sys
+    from conftest import PACKAGE_ROOT
+    program = """
+import torch
+from ictc_o3.ops.block_norm import block_norm_status, residual_block_norm
+x = torch.randn(50, 72, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    held = residual_block_norm(x, x, channels=8, lmax=2, norm=True)
+graph.replay()
+assert all(torch.equal(a, b) for a, b in zip(held, residual_block_norm(x, x, channels=8, lmax=2, norm=True)))
+assert block_norm_status() == 0
+print("same")
+"""
+    run = subprocess.run([sys.executable, "-c", program], env={**os.environ, "PYTHONPATH": PACKAGE_ROOT},
+                         capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
