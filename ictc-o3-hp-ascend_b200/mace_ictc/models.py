@@ -288,6 +288,8 @@ class ProductBlock(nn.Module):
 class MACEICTC(nn.Module):
     """MACE-ICTC energy model; ``energy(...)`` and ``energy_and_forces(...)``."""
 
+    block_norm = False      # also of models pickled before there were block norms
+
     def __init__(self, *, num_elements=None, channels=64, lmax=2, num_interactions=2, correlation=3, r_max=5.0,
                  num_basis=8, polynomial_cutoff_p=5, avg_num_neighbors=1.0, readout_hidden=16, ops=None,
                  atomic_numbers=(1, 6, 8), first_layer_self_connection=True, radial_sqrt_num_basis=False,
@@ -443,9 +445,10 @@ class MACEICTC(nn.Module):
         count = len(self.interactions) if layers is None else layers
         normed = self._block_start(h) if self.block_norm else None
         for layer in range(count):
-            message, sc = self.interactions[layer](self.ops, h if normed is None else normed, harmonics, feats, src,
+            norms = {"stream": h} if self.block_norm else {}
+            message, sc = self.interactions[layer](self.ops, normed if self.block_norm else h, harmonics, feats, src,
                                                    dst, mask, groups, owned, own_species,
-                                                   exchange=exchange if layer else None, stream=h)
+                                                   exchange=exchange if layer else None, **norms)
             mark(f"layer{layer}.interaction")
             if self.block_norm:
                 h, normed = self._block_end(layer, message, sc, own_species)
