@@ -86,6 +86,19 @@ PyObject* changed(PyObject*, PyObject* const* args, Py_ssize_t n) {
   Py_RETURN_NONE;
 }
 
+// holds(whole, from, part): whether the items of list `part` are those of list `whole` from `from` on.
+PyObject* holds(PyObject*, PyObject* const* args, Py_ssize_t n) {
+  if (n != 3 || !PyList_Check(args[0]) || !PyList_Check(args[2])) {
+    PyErr_SetString(PyExc_TypeError, "holds takes a list, an integer and a list");
+    return nullptr;
+  }
+  const Py_ssize_t from = PyLong_AsSsize_t(args[1]), count = PyList_GET_SIZE(args[2]);
+  if (PyErr_Occurred()) return nullptr;
+  bool same = from >= 0 && from <= PyList_GET_SIZE(args[0]) - count;
+  for (Py_ssize_t i = 0; same && i < count; ++i) same = PyList_GET_ITEM(args[0], from + i) == PyList_GET_ITEM(args[2], i);
+  return PyBool_FromLong(same);
+}
+
 // accumulates_on_default_stream(leaf): whether the leaf's gradient is added up on the device's default
 // stream, as it is while a graph recorded there lives.
 PyObject* accumulates_on_default_stream(PyObject*, PyObject* leaf) {
@@ -108,6 +121,8 @@ PyMethodDef methods[] = {
      "Addresses of tensors and their gradients."},
     {"changed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(changed)), METH_FASTCALL,
      "Raise the tensors' version counters."},
+    {"holds", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(holds)), METH_FASTCALL,
+     "Whether a list holds another one's items."},
     {"accumulates_on_default_stream", accumulates_on_default_stream, METH_O,
      "Whether a leaf's gradient is added up on the default stream."},
     {nullptr, nullptr, 0, nullptr}};

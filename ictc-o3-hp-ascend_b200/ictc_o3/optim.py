@@ -8,6 +8,7 @@ and EMA, ``mace_ictc/training/train_loop.py``).
 from __future__ import annotations
 
 import math
+import operator
 from array import array
 
 import torch
@@ -142,6 +143,19 @@ class AdamW(torch.optim.Optimizer):
 
     # -- one step -----------------------------------------------------------
 
+    def _check_groups(self):
+        """The tables and host arrays are those of the parameters at construction."""
+        first = 0
+        for group in self.param_groups:
+            part = group["params"]
+            same = (self._host.holds(self._params, first, part) if self._host is not None and type(part) is list else
+                    len(part) <= len(self._params) - first and all(map(operator.is_, self._params[first:], part)))
+            if not same:
+                break
+            first += len(part)
+        if first != len(self._params) or not same:
+            raise ValueError("the parameters of the groups are fixed when the optimizer is built")
+
     def _gather(self):
         """Fill the arrays of addresses (0: no gradient); returns how many have a gradient, and
         temporaries that must outlive the launch."""
@@ -173,6 +187,7 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        self._check_groups()
         groups = [_hyperparameters(group) for group in self.param_groups]
         live, kept = self._gather()
         if not live:

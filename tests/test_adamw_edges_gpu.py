@@ -236,3 +236,31 @@ def test_negated_parameters_are_refused(cuda_device):
     p.grad = torch.ones(5, device=cuda_device)
     with pytest.raises(ValueError, match="has changed"):
         opt.step()
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_changed_groups_are_refused(native, cuda_device, monkeypatch):
+    """Addresses lie in arrays of the parameters at construction: other lists must not be read from them."""
+    from ictc_o3.backends.cuda import _native
+    from ictc_o3.optim import AdamW
+
+    def missing():
+        raise _native.NativeError("not built")
+
+    if not native:
+        monkeypatch.setattr(_native, "host_tensors", missing)
+    a, b, c, d = make([30, 5, 7, 5], cuda_device)
+    opt = AdamW([{"params": [a, b]}, {"params": [c], "lr": 1e-2}])
+    opt.step()
+    kept = snapshot(opt, [a, b, c])
+    first, second = opt.param_groups
+    for groups in ([{**first, "params": [a, b, d]}, second], [{**first, "params": [a]}, second], [first], [second, first],
+                   [{**first, "params": [a, d]}, second], [first, second, {**second, "params": [d]}],
+                   [first, {**second, "params": []}], [first, {**second, "params": [c, d, d, d]}], []):
+        opt.param_groups = groups
+        with pytest.raises(ValueError, match="fixed"):
+            opt.step()
+        assert all(torch.equal(x, y) for x, y in zip(kept, snapshot(opt, [a, b, c])))
+    opt.param_groups = [{**first, "params": (a, b)}, second]      # the same ones in another container
+    opt.step()
+    assert int(opt.state[c]["step"]) == 2
