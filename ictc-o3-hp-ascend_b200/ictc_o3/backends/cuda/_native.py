@@ -147,17 +147,18 @@ def host_tensors():
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
-def _address(tensor, name):
+_Tensor = torch.Tensor
+
+
+def _no_address(name):
     # a host tensor in the place of a number (a size under torch.jit.trace) would pass its address as that number
-    if not tensor.is_cuda:
-        raise TypeError(f"{name} takes addresses of CUDA tensors only")
-    return tensor.data_ptr()
+    raise TypeError(f"{name} takes addresses of CUDA tensors only")
 
 
 def launch(device, name, *args):
     """``call`` with ``device`` current and its current stream as the last argument; CUDA tensors may be
     given for their addresses (None: NULL)."""
-    args = [_address(a, name) if isinstance(a, torch.Tensor) else a for a in args]
+    args = [(a.data_ptr() if a.is_cuda else _no_address(name)) if isinstance(a, _Tensor) else a for a in args]
     if torch.cuda.current_device() != device.index:
         with torch.cuda.device(device):
             return launch(device, name, *args)

@@ -29,6 +29,9 @@ __all__ = ["degree_norm", "residual_block_norm", "DegreeNorm", "ResidualBlockNor
            "block_norm_status"]
 
 
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
+
+
 @functools.lru_cache(maxsize=256, typed=True)
 def _form(channels, lmax, layout, eps, norm):
     if not isinstance(channels, int) or isinstance(channels, bool) or channels < 1:
@@ -45,7 +48,7 @@ def _form(channels, lmax, layout, eps, norm):
 
 
 def _check(form, rows, weights, gate=None):
-    if torch.jit.is_tracing():      # sizes are tensors there, and a trace would hold the outputs' allocation alone
+    if _is_tracing():      # sizes are tensors there, and a trace would hold the outputs' allocation alone
         raise ValueError("block norms cannot be traced; the CUDA backend requires ordinary eager autograd")
     c, degrees = form.channels, form.lmax + 1
     n = rows[0].shape[0] if rows[0].ndim else 0
