@@ -264,3 +264,26 @@ def test_changed_groups_are_refused(native, cuda_device, monkeypatch):
     opt.param_groups = [{**first, "params": (a, b)}, second]      # the same ones in another container
     opt.step()
     assert int(opt.state[c]["step"]) == 2
+
+
+def test_8_bit_codes_with_clipping_are_exact(cuda_device):
+    """The clip factor that the first kernel left is one more FP32 product: codes equal the restatement's."""
+    from ictc_o3.optim import AdamW
+    from test_adamw_gpu import random_state
+    params = make([1, 255, 257, 9001], cuda_device, seed=91)
+    total = float(torch.cat([p.grad.double() for p in params]).norm())
+    opt = AdamW(params, **HYPER, state_bits=8, max_norm=0.3 * total, seed=77)
+    before = random_state(opt, 3)
+    opt.step()
+    clip = opt._table.workspace[12:16].view(torch.float32).cpu()
+    assert abs(float(clip) - 0.3 * total / (total + 1e-6)) <= 4 * adamw_oracle.U
+    b1, b2 = (torch.tensor(b, dtype=torch.float32) for b in HYPER["betas"])
+    c1, c2 = (torch.tensor(1 - b, dtype=torch.float32) for b in HYPER["betas"])
+    for p, (steps, start, m, v) in zip(params, before):
+        g = p.grad.cpu() * clip
+        r_m, r_v = adamw_oracle.random_bits(start, p.numel(), steps + 1, opt.seed)
+        for key, x, r, signed in (("exp_avg", m.float() * b1 + g * c1, r_m, True),
+                                  ("exp_avg_sq", v.float() * b2 + (g * g) * c2, r_v, False)):
+            codes, byte = adamw_oracle.encode(x.reshape(-1), r, signed)
+            assert torch.equal(opt.state[p][key].cpu().view(-1), codes)
+            assert torch.equal(opt.state[p][key + "_exponent"].cpu(), byte)
