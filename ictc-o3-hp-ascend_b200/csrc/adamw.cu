@@ -12,7 +12,7 @@
 // in the kernel's parameters (they may change from step to step).  One block per chunk,
 // which it works off in turns of 1,024 values, eight per thread; how many turns a chunk
 // has goes by the total (the caller's rule): one where there are few values, since
-// latency counts, 16 where there are many, since a block's own costs then spread.
+// latency counts, 8 where there are many, since a block's own costs then spread.
 //
 // 8-bit moments: blocks of 256 values (one warp's share) have a power-of-two scale
 // 2^(byte - 127), byte = exponent field of the block's largest magnitude + 1, limited to
@@ -25,16 +25,20 @@
 // stored value at all.  16 random bits each from Philox4x32-7 (Salmon, Moraes, Dror,
 // Shaw: Parallel random numbers: as easy as 1, 2, 3, 2011), counter (index of the four
 // values, t), key = seed: the codes are a function of the inputs alone.  A positive v
-// never rounds to zero (the weight's step divides by sqrt(v)).  A block whose new moments
+// never rounds to code zero (the weight's step divides by sqrt(v); in blocks whose scale is below 2^-119 the least
+// codes' values leave FP32's range and are zero all the same: largest gradients of some 1e-17).  A block whose new moments
 // are not all finite is left as it was, its weights too: the codes hold no NaN.
 // Every product of the moments is rounded by itself (no FMA contraction), so the codes
 // do not depend on how the compiler pairs operations.
 //
 // Measured on a B200 (copy rate 6,565 GB/s), 160 M values in 230 tensors: 32-bit step 674 us
-// (28 B per value: 6,650 GB/s), with average 865 us (36 B: 6,650 GB/s): bound by memory.
-// 8-bit step 549 us (16 B: 4,660 GB/s), with average 693 us: bound by its 80 instructions per value (a
-// fifth of them Philox), issue slots 63% taken.  Gradient norm 108 us (4 B: 5,900 GB/s).  Decoding 160 us (6 B:
-// 6,000 GB/s).  30,000 values in 42 tensors: 8 us (6 us with 8 bits), launch and latency.
+// (28 B per value: 6,650 GB/s), with average 870 us (36 B: 6,620 GB/s): bound by memory.  (Above the copy's
+// rate: the memory serves four reads per three writes faster than one per one; torch's addition of two arrays reaches
+// 6,990 GB/s here, its copy 6,610.)  8-bit step 545 us (16 B: 4,700 GB/s), with average 701 us: neither memory (half
+// of its rate) nor issue slots (63% taken, 80 instructions per value, a fifth of them Philox) are full; warps
+// wait for their loads, since 20 warps per multiprocessor have no registers left to read ahead.  Gradient norm 108 us
+// (4 B: 5,930 GB/s).  Decoding 148 us (6 B: 6,490 GB/s).  30,000 values in 42 tensors: 8 us (6 us with 8 bits), launch
+// and latency.
 #include "ictc_cuda.h"
 
 #include <cstdint>
@@ -395,8 +399,8 @@ __device__ __forceinline__ void update(const Turn<BITS, AVERAGE>& x, const Args&
 }
 
 // Blocks per multiprocessor.  32-bit states are bound by memory: the next turn's values are on their way
-// while one is worked on (160 M values, 16 turns: 683 us, 100% of the copy rate; one turn per block 718 us).
-// 8-bit ones are bound by instructions: five blocks hold their values without spills (4: 585, 5: 539, 7: 613 us).
+// while one is worked on (160 M values, 8 turns: 673 us, one turn per block 859 us).
+// 8-bit ones keep most warps with five blocks and few spills (4: 585, 5: 539, 7: 613 us, one after another).
 constexpr int kResident32 = 4, kResident8 = 5;
 template <int BITS, bool AVERAGE>
 __global__ void __launch_bounds__(kThreads, BITS == 8 ? kResident8 : kResident32)

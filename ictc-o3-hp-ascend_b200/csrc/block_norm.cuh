@@ -34,10 +34,16 @@
 // a fixed order: no atomics, the same bits every time.
 //
 // Measured on a B200 (copy rate 6,565 GB/s; bytes: every row array once), with gate:
-//   262,144 rows of C64/lmax 2: forward 438 us (5,970 GB/s), backward with weights 653 us (6,160),
-//   second 1,265 us (5,250);  8,192 rows of C128/lmax 3: 53 us (5,360), 84 us (5,200), 176 us (4,100);
-//   100,000 rows of C128/lmax 0: 76 us (3,380), 104 us (3,920), 221 us (3,010).
-// The forward and the first gradients are near the memory's rate.  The second derivatives at lmax 3 stage 53 KB per
+//   262,144 rows of C64/lmax 2: forward 436 us (6,010 GB/s), backward with weights 647 us (6,220),
+//   second 1,250 us (5,320);  8,192 rows of C128/lmax 3: 51 us (5,620), 80 us (5,420), 175 us (4,120);
+//   50,000 rows of C132/lmax 1: 91 us (5,210), 162 us (4,570), 392 us (3,100);
+//   100,000 rows of C128/lmax 0: 63 us (4,040), 101 us (4,050), 218 us (3,050);
+//   without bulk copies (addresses off by one value): C64/lmax 2 642 us, 1,013 us, 2,098 us; C128/lmax 3
+//   80 us, 134 us, 292 us; C132/lmax 1 156 us, 248 us, 556 us; 32,768 rows of C50/lmax 2 93 us (2,740), 151 us, 286 us;
+//   wide rows (HOLD false: more than 512 channels, 384 or 256 in some derivatives): 20,000 rows of C512/lmax 1 173 us
+//   (4,260), 257 us (4,460), 1,283 us (1,470); 4,000 rows of C450/lmax 3 106 us (4,640), 314 us (2,390), 516 us (2,400);
+//   20,000 rows of C1028/lmax 0 597 us (690), 779 us (840), 1,119 us (960).
+// The forward and the first gradients are near the memory's rate at lmax 2 and 3.  The second derivatives at lmax 3 stage 53 KB per
 // row of C128, so two rows are worked on and two are under way per multiprocessor: eight warps, bound by the
 // latency of their instructions (issue slots 37% taken; with no row written and half of the inputs 600 of 646 us
 // at 32,768 rows).  Two sets of warps per row, one for degree 3 and one for the rest, gave 615 us there but lost at

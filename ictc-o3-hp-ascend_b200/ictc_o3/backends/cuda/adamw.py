@@ -14,7 +14,7 @@ from . import _native
 from ._native import launch
 
 BLOCK = 256   # values that share a scale of the 8-bit moments (csrc/adamw.cu)
-WAVE = 740    # blocks that a B200 holds at once
+WAVE = 740    # blocks of the 8-bit kernel that a B200 holds at once (five per multiprocessor; four of the 32-bit one)
 
 
 def blocks_of(numel: int) -> int:
@@ -25,9 +25,9 @@ def turns_of(total: int) -> int:
     """Turns of 1,024 values per block: as many as leave one wave of blocks, 8 at most.
 
     Microseconds of a step with 32 / 8-bit states and 1, 2, 4, 8, 16 turns:
-    30,000 values 8.3 10.1 10.3 13.3 19.2 / 6.2 8.3 10.3 12.4 18.5;  1 M 12.4 10.3 12.1 14.4 20.9 / 11.0
-    10.3 10.3 14.4 20.5;  4 M 24.9 20.4 20.2 18.5 22.6 / 24.8 20.6 20.4 20.7 24.4;  16 M 95 79 77 76 78 / 91
-    74 67 66 74;  160 M 879 689 664 674 678 / 843 656 580 538 529."""
+    30,000 values 8.3 8.6 10.4 12.5 18.6 / 6.3 8.4 10.3 12.4 18.6;  1 M 12.4 10.4 11.5 14.5 20.6 / 11.1
+    10.4 10.4 14.5 20.6;  4 M 24.6 20.0 20.2 18.4 22.7 / 24.7 20.6 20.6 21.2 24.7;  16 M 94 77 76 76 78 / 90
+    74 67 67 75;  160 M 859 684 663 673 678 / 828 655 584 542 532."""
     turns = 1
     while turns < 8 and total > turns * 1024 * WAVE:
         turns *= 2

@@ -58,6 +58,8 @@ class AdamW(torch.optim.Optimizer):
     them makes that factor NaN (moments in 8 bits, and their weights, then stay as they were).
     ``skip_nonfinite``: a step with an infinite or NaN gradient changes nothing and is not counted.
     ``ema_decay``: keeps average = d average + (1 - d) weight in ``state[p]["ema"]``.
+    ``state[p]`` holds views of the buffers that the kernels use: values may be written into them, not put
+    in their place.
 
     ``step`` never waits for the device, allocates nothing for contiguous gradients and may be
     captured into a CUDA graph; addresses and hyperparameters are then those of the
@@ -225,8 +227,9 @@ class AdamW(torch.optim.Optimizer):
 
     def moments(self):
         """(exp_avg, exp_avg_sq) of all parameters one after another, each from a multiple of 256
-        values on with zeros between: the state's own FP32 buffers, or the values (BF16, exact)
-        that 8-bit states stand for."""
+        values on with zeros between: the state's own FP32 buffers, or the values that 8-bit states
+        stand for (BF16; exact where a block's scale is at least 2^-99: below, its least codes leave
+        BF16's range)."""
         if self.state_bits == 32:
             return self._flat["m"], self._flat["v"]
         return self._table.decode(self._flat)

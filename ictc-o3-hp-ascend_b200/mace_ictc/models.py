@@ -310,8 +310,8 @@ class MACEICTC(nn.Module):
         into a model of either.
 
         ``block_norm`` adds norms before and after every block with a gate and a residual
-        scale that starts at ``block_scale`` (``ictc_o3.ops.block_norm``), for stacks whose
-        activations would grow from layer to layer.  Such a model is this package's own:
+        scale that starts at ``block_scale`` (``ictc_o3.ops.block_norm``): each block then reads
+        rows of size one per degree, whatever the layers before it made of them.  Such a model is this package's own:
         reference checkpoints neither load into it nor are written from it."""
         super().__init__()
         if product_backend not in PRODUCT_MODULES:
