@@ -25,15 +25,12 @@ def _positive_int(value, name):
 
 def create_model(*, channels=64, lmax=3, edge_lmax=None, num_interactions=2, correlation=3, use_reduced_cg=False,
                  atomic_numbers=(1, 6, 8), cutoff=5.0, avg_num_neighbors=50.0, device="cuda",
-                 dtype=torch.float32, electrostatics=None, block_norm=False, block_scale=1.0):
+                 dtype=torch.float32, electrostatics=None):
     """A freshly initialised MACE-ICTC model on the CUDA backend (not a trained potential).
 
     Bridge-U product blocks, as the reference's factory builds (its couplings are the
-    ICTC ones until a reference checkpoint is loaded).  ``block_norm`` and ``block_scale``
-    are the model's: norms before and after every block, which the reference does not have."""
+    ICTC ones until a reference checkpoint is loaded)."""
     from .models import MACEICTC
-    if not isinstance(block_norm, bool):
-        raise TypeError("block_norm must be a boolean")
     _positive_int(num_interactions, "num_interactions")
     _positive_int(channels, "channels")
     _positive_int(correlation, "correlation")
@@ -54,7 +51,7 @@ def create_model(*, channels=64, lmax=3, edge_lmax=None, num_interactions=2, cor
         raise ValueError("the CUDA backend runs FP32 models on CUDA devices")
     model = MACEICTC(channels=channels, lmax=lmax, num_interactions=num_interactions, correlation=correlation,
                      r_max=cutoff, avg_num_neighbors=avg_num_neighbors, atomic_numbers=atomic_numbers,
-                     product_backend="ictd-bridge-u", block_norm=block_norm, block_scale=block_scale)
+                     product_backend="ictd-bridge-u")
     return model.to(device)
 
 
