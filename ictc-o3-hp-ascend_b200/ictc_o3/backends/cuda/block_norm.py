@@ -199,7 +199,7 @@ class _Block(torch.autograd.Function):
         form = ctx.form
         _check_capture(ctx)
         _refuse_tangents(*cotangents)
-        stream, branch, gate, post, scale, pre = ctx.saved_tensors
+        stream, branch, gate, post, scale, pre = saved = ctx.saved_tensors      # once: checkpoints recompute per access
         p = cotangents[0] if branch is not None else None
         q = cotangents[-1] if form.norm else None
         if p is None and q is None:
@@ -210,7 +210,7 @@ class _Block(torch.autograd.Function):
         # views that could be asked cost 25 us of host time)
         _, need_stream, need_branch, need_gate, *need_weights = ctx.needs_input_grad
         nodes = iter([node for node, _ in ctx.next_functions])      # of the tensors among the arguments
-        _, at_branch, _, *at_weights = [None if t is None else next(nodes) for t in ctx.saved_tensors]
+        _, at_branch, _, *at_weights = [None if t is None else next(nodes) for t in saved]
         need_branch = need_branch and _runs(at_branch)
         runs = any(n and _runs(node) for n, node in zip(need_weights, at_weights))
         need = (need_stream, need_branch, need_gate, *[n and runs for n in need_weights])

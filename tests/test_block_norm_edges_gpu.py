@@ -162,3 +162,25 @@ print("same")
     run = subprocess.run([sys.executable, "-c", program], env={**os.environ, "PYTHONPATH": PACKAGE_ROOT},
                          capture_output=True, text=True, timeout=300)
     assert run.returncode == 0 and "same" in run.stdout, run.stderr[-2000:]
+
+
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_blocks(reentrant, cuda_device):
+    """Recomputed in the backward pass: the same gradients, and the same adjoints of theirs."""
+    from torch.utils.checkpoint import checkpoint
+    t = inputs(23, 12, 2, seed=3)
+    leaves = [t[k] for k in NAMES]
+
+    def whole(*args):
+        return call(dict(zip(NAMES, args)))
+
+    if reentrant:       # this form has first gradients alone, into .grad
+        want = torch.autograd.grad(call(t), leaves, [t["p"], t["q"]])
+        torch.autograd.backward(checkpoint(whole, *leaves, use_reentrant=True), [t["p"], t["q"]])
+        assert all(torch.equal(x.grad, w) for x, w in zip(leaves, want))
+        return
+    want = all_of(t)
+    out = checkpoint(whole, *leaves, use_reentrant=False)
+    first = torch.autograd.grad(out, leaves, [t["p"], t["q"]], create_graph=True)
+    second = torch.autograd.grad(first[:3], [*leaves, t["p"], t["q"]], [t["d_stream"], t["d_branch"], t["d_gate"]])
+    assert all(torch.equal(a, b) for a, b in zip((*out, *first, *second), want))
