@@ -34,8 +34,8 @@
 // Measured on a B200 (copy rate 6,565 GB/s), 160 M values in 230 tensors: 32-bit step 674 us
 // (28 B per value: 6,650 GB/s), with average 870 us (36 B: 6,620 GB/s): bound by memory.  (Above the copy's
 // rate: the memory serves four reads per three writes faster than one per one; torch's addition of two arrays reaches
-// 6,990 GB/s here, its copy 6,610.)  8-bit step 545 us (16 B: 4,700 GB/s), with average 701 us: neither memory (half
-// of its rate) nor issue slots (63% taken, 80 instructions per value, a fifth of them Philox) are full; warps
+// 6,990 GB/s here, its copy 6,610.)  8-bit step 545 us (16 B: 4,700 GB/s), with average 701 us: neither memory (72%
+// of the copy's rate) nor issue slots (63% taken, 80 instructions per value, a fifth of them Philox) are full; warps
 // wait for their loads, since 20 warps per multiprocessor have no registers left to read ahead.  Gradient norm 108 us
 // (4 B: 5,930 GB/s).  Decoding 148 us (6 B: 6,490 GB/s).  30,000 values in 42 tensors: 8 us (6 us with 8 bits), launch
 // and latency.

@@ -245,7 +245,7 @@ class AdamW(torch.optim.Optimizer):
         ``skip_nonfinite`` and ``ema_decay`` belong to the constructor."""
         state_dict = super().state_dict()
         # dicts of their own: a value replaced in the optimizer's would part it from the buffers that the kernels use
-        state_dict["state"] = {k: dict(v) for k, v in state_dict["state"].items()}
+        state_dict["state"] = {k: dict(v) if isinstance(v, dict) else v for k, v in state_dict["state"].items()}
         if self.state_bits == 8:
             state_dict["seed"] = self.seed
         return state_dict

@@ -287,3 +287,16 @@ def test_8_bit_codes_with_clipping_are_exact(cuda_device):
             codes, byte = adamw_oracle.encode(x.reshape(-1), r, signed)
             assert torch.equal(opt.state[p][key].cpu().view(-1), codes)
             assert torch.equal(opt.state[p][key + "_exponent"].cpu(), byte)
+
+
+def test_state_of_a_users_own(cuda_device):
+    """What a user keeps in the optimizer's state beside the tensors' entries travels with the state dict."""
+    from ictc_o3.optim import AdamW
+    opt = AdamW(make([30], cuda_device))
+    opt.state["epoch"] = 3
+    opt.step()
+    saved = opt.state_dict()
+    assert saved["state"]["epoch"] == 3 and set(saved["state"][0]) == {"step", "exp_avg", "exp_avg_sq"}
+    opt.load_state_dict(saved)
+    opt.step()
+    assert int(opt.state[opt.param_groups[0]["params"][0]]["step"]) == 2
